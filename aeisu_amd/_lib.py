@@ -24,9 +24,20 @@ LAYOUT_F16, LAYOUT_F32 = 0, 1
 FLAG_KEEP_INTERMEDIATES, FLAG_STAGE_TIMING, FLAG_NO_PAD, FLAG_UNFUSED, FLAG_BODY_TILE24 = 1, 2, 4, 8, 16
 FLAG_BODY_NO_EXCHANGE, FLAG_BODY_EXCHANGE_FALLBACK = 32, 64
 BUF_SKIP, BUF_LOW0, BUF_WORK, BUF_META = 0, 1, 6, 7
+TYPE_F16, TYPE_F32, TYPE_BF16, TYPE_E4M3 = 0, 1, 2, 3
 STAGES = ("project", "compress", "bottleneck", "expand", "refine_tail", "head", "total")
 
 _P, _I, _U, _S = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint, ctypes.c_size_t
+_L, _F = ctypes.c_int64, ctypes.c_float
+
+
+class Product(ctypes.Structure):
+    """aeisu_product"""
+    _fields_ = [("type", _I), ("out_type", _I), ("rows", _L), ("n", _L), ("k", _L), ("x", _P), ("x_stride", _L),
+                ("x_scales", _P), ("x_scales_stride", _L), ("w", _P), ("w_stride", _L), ("w_expert_stride", _L),
+                ("w_scales", _P), ("bias", _P), ("slope", _F), ("out", _P), ("out_stride", _L)]
+
+
 SIGNATURES = {
     "aeisu_create_from_file": (_I, [ctypes.c_char_p, _I, ctypes.POINTER(_P)]),
     "aeisu_create_from_memory": (_I, [_P, _S, _I, ctypes.POINTER(_P)]),
@@ -49,6 +60,10 @@ SIGNATURES = {
     "aeisu_persistent_bytes": (_S, [_P]),
     "aeisu_artifact_checksum": (_I, [_P, ctypes.c_char_p]),
     "aeisu_destroy": (None, [_P]),
+    "aeisu_quantize_rows": (_I, [_P, _I, _L, _L, _L, _I, _P, _L, _P, _L, _P, _L, _P]),
+    "aeisu_quantize_weight": (_I, [_P, _I, _L, _L, _L, _L, _L, _P, _P, _P]),
+    "aeisu_matmul": (_I, [_P, _P]),
+    "aeisu_grouped_matmul": (_I, [_P, _P, _L, _P]),
     "aeisu_last_error": (ctypes.c_char_p, []),
     "aeisu_version": (ctypes.c_char_p, []),
 }

@@ -1,0 +1,134 @@
+// C entry points of the block-scaled operators: argument checks, then one launch.
+#include "blocks.hpp"
+
+#include <cmath>
+#include <string>
+
+#include "error.hpp"
+
+namespace aeisu {
+namespace {
+
+constexpr int64_t kMost = int64_t(1) << 30;        // rows, columns and experts of an operand
+constexpr int64_t kMostStride = int64_t(1) << 40;  // elements between rows or experts
+
+void require(bool ok, const char* what) {
+  if (!ok) fail(AEISU_ERR_INVALID_ARGUMENT, what);
+}
+bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+size_t size_of(int type) {
+  switch (type) {
+    case AEISU_TYPE_F16:
+    case AEISU_TYPE_BF16: return 2;
+    case AEISU_TYPE_F32: return 4;
+    case AEISU_TYPE_E4M3: return 1;
+    default: fail(AEISU_ERR_INVALID_ARGUMENT, "unknown element type");
+  }
+}
+void require_extent(int64_t v, const char* what) { require(v >= 0 && v < kMost, what); }
+// a row stride: at least the row, unless there is no second row
+void require_stride(int64_t stride, int64_t row, int64_t rows, const char* what) {
+  require(stride <= kMostStride && stride >= 0 && (rows <= 1 || stride >= row), what);
+}
+
+void check_product(const aeisu_product& p, int64_t experts) {
+  require(p.type == AEISU_TYPE_E4M3 || p.type == AEISU_TYPE_F16 || p.type == AEISU_TYPE_BF16,
+          "product: operands are E4M3, FP16 or BF16");
+  require(p.out_type == AEISU_TYPE_F16 || p.out_type == AEISU_TYPE_BF16 || p.out_type == AEISU_TYPE_F32,
+          "product: results are FP16, BF16 or FP32");
+  require_extent(p.rows, "product: rows out of range");
+  require_extent(p.n, "product: n out of range");
+  require_extent(p.k, "product: k out of range");
+  require(std::isfinite(p.slope) && p.slope >= 0.f, "product: the slope is finite and not negative");
+  if (p.rows == 0 || p.n == 0) return;
+  const bool e4m3 = p.type == AEISU_TYPE_E4M3;
+  const size_t es = size_of(p.type), os = size_of(p.out_type);
+  const int64_t kp = e4m3 ? kBlock * blocks_of(p.k) : p.k;
+  require(p.out && aligned(p.out, os), "product: null or misaligned result");
+  require_stride(p.out_stride, p.n, p.rows, "product: the result's row stride is below n");
+  require(!p.bias || aligned(p.bias, 4), "product: misaligned bias");
+  if (p.k == 0) return;
+  require(p.x && p.w && aligned(p.x, es) && aligned(p.w, es), "product: null or misaligned operand");
+  require_stride(p.x_stride, kp, p.rows, "product: x's row stride is below its (padded) columns");
+  require_stride(p.w_stride, kp, p.n, "product: w's row stride is below its (padded) columns");
+  require(p.w_expert_stride >= 0 && p.w_expert_stride <= kMostStride, "product: w's expert stride is out of range");
+  if (e4m3) {
+    require(aligned(p.x, 16) && aligned(p.w, 16) && p.x_stride % 16 == 0 && p.w_stride % 16 == 0 &&
+                (experts <= 1 || p.w_expert_stride % 16 == 0),
+            "product: rows of E4M3 codes are 16-byte aligned");
+    require(p.x_scales && p.w_scales && aligned(p.x_scales, 4) && aligned(p.w_scales, 4), "product: null or misaligned scales");
+    require_stride(p.x_scales_stride, p.rows, blocks_of(p.k), "product: the stride of x's scales is below rows");
+  }
+}
+
+void run_product(const aeisu_product* p, const int32_t* offsets, int64_t experts, void* stream) {
+  require(p != nullptr, "null product");
+  check_product(*p, experts);
+  if (p->rows == 0 || p->n == 0) return;
+  check_launch(launch_product(*p, offsets, int(experts), (hipStream_t)stream), "product", (hipStream_t)stream);
+}
+
+}  // namespace
+}  // namespace aeisu
+
+using namespace aeisu;
+
+extern "C" {
+
+int aeisu_quantize_rows(const void* d_x, int type, int64_t x_rows, int64_t x_stride, int64_t cols, int gated,
+                        const int32_t* d_index, int64_t rows, void* d_codes, int64_t codes_stride, float* d_scales,
+                        int64_t scales_stride, void* stream) {
+  return guarded([&] {
+    require(type == AEISU_TYPE_F16 || type == AEISU_TYPE_BF16 || type == AEISU_TYPE_F32,
+            "quantize: values are FP16, BF16 or FP32");
+    require_extent(x_rows, "quantize: x_rows out of range");
+    require_extent(rows, "quantize: rows out of range");
+    require_extent(cols, "quantize: cols out of range");
+    require(d_index || rows <= x_rows, "quantize: more rows than x has and no index");
+    if (rows == 0 || cols == 0) return;
+    const int64_t kp = kBlock * blocks_of(cols);
+    require(x_rows == 0 || (d_x && aligned(d_x, size_of(type))), "quantize: null or misaligned x");
+    require_stride(x_stride, gated ? 2 * cols : cols, x_rows, "quantize: x's row stride is below its columns");
+    require(!d_index || aligned(d_index, 4), "quantize: misaligned index");
+    require(d_codes && aligned(d_codes, 16) && codes_stride % 16 == 0, "quantize: rows of codes are 16-byte aligned");
+    require(codes_stride >= kp && codes_stride <= kMostStride, "quantize: the codes' row stride is below the padded columns");
+    require(d_scales && aligned(d_scales, 4), "quantize: null or misaligned scales");
+    require_stride(scales_stride, rows, blocks_of(cols), "quantize: the scales' stride is below rows");
+    const QuantizeRows q{d_x,  x_rows, x_stride, cols, d_index, rows, static_cast<uint8_t*>(d_codes), codes_stride,
+                         d_scales, scales_stride};
+    check_launch(launch_quantize_rows(q, type, gated != 0, (hipStream_t)stream), "quantize_rows", (hipStream_t)stream);
+  });
+}
+
+int aeisu_quantize_weight(const void* d_w, int type, int64_t experts, int64_t n, int64_t k, int64_t expert_stride,
+                          int64_t row_stride, void* d_codes, float* d_scales, void* stream) {
+  return guarded([&] {
+    require(type == AEISU_TYPE_F16 || type == AEISU_TYPE_BF16 || type == AEISU_TYPE_F32,
+            "quantize: values are FP16, BF16 or FP32");
+    require(experts >= 0 && experts <= 65535, "quantize: experts out of range");
+    require_extent(n, "quantize: n out of range");
+    require_extent(k, "quantize: k out of range");
+    if (experts == 0 || n == 0 || k == 0) return;
+    require(d_w && aligned(d_w, size_of(type)), "quantize: null or misaligned weights");
+    require_stride(row_stride, k, n, "quantize: the weights' row stride is below k");
+    require(expert_stride >= 0 && expert_stride <= kMostStride, "quantize: the expert stride is out of range");
+    require(d_codes && aligned(d_codes, 16), "quantize: codes are 16-byte aligned");
+    require(d_scales && aligned(d_scales, 4), "quantize: null or misaligned scales");
+    const QuantizeWeight q{d_w, n, k, expert_stride, row_stride, static_cast<uint8_t*>(d_codes), d_scales};
+    check_launch(launch_quantize_weight(q, type, experts, (hipStream_t)stream), "quantize_weight", (hipStream_t)stream);
+  });
+}
+
+int aeisu_matmul(const aeisu_product* p, void* stream) {
+  return guarded([&] { run_product(p, nullptr, 1, stream); });
+}
+
+int aeisu_grouped_matmul(const aeisu_product* p, const int32_t* d_offsets, int64_t experts, void* stream) {
+  return guarded([&] {
+    require(experts >= 1 && experts <= 65535, "grouped product: 1 to 65535 experts");
+    require(d_offsets && aligned(d_offsets, 4), "grouped product: null or misaligned offsets");
+    run_product(p, d_offsets, experts, stream);
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,36 @@
+// Launches of the block-scaled operators (k_quantize.hip, k_product.hip); arguments are checked in blocks.cpp.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "aeisu_amd.h"
+
+namespace aeisu {
+
+constexpr int kBlock = 128;              // columns that share a scale
+constexpr int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }
+
+struct QuantizeRows {
+  const void* x;
+  int64_t x_rows, x_stride, cols;
+  const int32_t* index;
+  int64_t rows;
+  uint8_t* codes;
+  int64_t codes_stride;
+  float* scales;
+  int64_t scales_stride;
+};
+hipError_t launch_quantize_rows(const QuantizeRows& q, int type, bool gated, hipStream_t stream);
+
+struct QuantizeWeight {
+  const void* w;
+  int64_t n, k, expert_stride, row_stride;
+  uint8_t* codes;
+  float* scales;
+};
+hipError_t launch_quantize_weight(const QuantizeWeight& q, int type, int64_t experts, hipStream_t stream);
+
+// offsets: null for one weight
+hipError_t launch_product(const aeisu_product& p, const int32_t* offsets, int experts, hipStream_t stream);
+
+}  // namespace aeisu

@@ -22,6 +22,7 @@
 #include <vector>
 
 #include "aeisu_amd.h"
+#include "error.hpp"
 #include "kernels.hpp"
 #include "sha256.hpp"
 
@@ -30,15 +31,6 @@ namespace aeisu {
 // ------------------------------------------------------------------------------------------------
 // errors
 // ------------------------------------------------------------------------------------------------
-struct Error : std::runtime_error {
-  int code;
-  Error(int c, const std::string& m) : std::runtime_error(m), code(c) {}
-};
-[[noreturn]] static void fail(int code, const std::string& msg) { throw Error(code, msg); }
-static void check_hip(hipError_t e, const char* what) {
-  if (e != hipSuccess) fail(AEISU_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
-}
-
 // Diagnostic, off by default (the reference's AESS_NEURAL_EAGER_VALIDATE, SrcPyrCudaRuntime.cu:5349-5354):
 // with AEISU_EAGER_VALIDATE=1 in the environment every kernel launch outside graph capture is followed
 // by a synchronisation of its stream, so that an asynchronous failure is reported with the launch
@@ -50,7 +42,7 @@ static bool eager_validate() {
   }();
   return on;
 }
-static void check_launch(hipError_t e, const char* what, hipStream_t s) {
+void check_launch(hipError_t e, const char* what, hipStream_t s) {
   check_hip(e, what);
   if (!eager_validate()) return;
   hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
@@ -1243,32 +1235,15 @@ static void enqueue_noalloc(const Runtime& rt, int batch, int height, int width,
 // ================================================================================================
 // C ABI
 // ================================================================================================
-using aeisu::Error;
 using aeisu::Runtime;
 
 struct aeisu_runtime {
   std::unique_ptr<Runtime> impl;
 };
 
-static thread_local std::string g_last_error;
-
-template <typename Fn>
-static int guarded(Fn fn) {
-  try {
-    fn();
-    g_last_error.clear();
-    return AEISU_OK;
-  } catch (const Error& e) {
-    g_last_error = e.what();
-    return e.code;
-  } catch (const std::bad_alloc&) {
-    g_last_error = "host allocation failed";
-    return AEISU_ERR_HIP;
-  } catch (const std::exception& e) {
-    g_last_error = e.what();
-    return AEISU_ERR_HIP;
-  }
-}
+thread_local std::string aeisu::g_last_error;
+using aeisu::g_last_error;
+using aeisu::guarded;
 
 static Runtime& runtime_of(aeisu_runtime* rt) {
   if (!rt || !rt->impl) aeisu::fail(AEISU_ERR_INVALID_ARGUMENT, "null runtime handle");
