@@ -1,0 +1,185 @@
+// Products in tiles of 128 x 128: four waves of 64 x 64, two blocks on a CU.
+#include "product.hpp"
+
+namespace aeisu {
+namespace {
+
+template <int TYPE, int OUT, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void product_tiles_kernel(aeisu_product p, const int32_t* offsets,
+                                                                                   int experts, int ntiles) {
+  constexpr bool kE4M3 = TYPE == AEISU_TYPE_E4M3, EXACT = OUT == AEISU_TYPE_F32;
+  constexpr int ES = kE4M3 ? 1 : 2, STEP = kStepBytes / ES;
+  constexpr int WAVES = (BM / WM) * (BN / WN), MT = WM / 16, NT = WN / 16;
+  constexpr int XC = BM / 8, CHUNKS = (BM + BN) / 8, CH = CHUNKS / WAVES;     // chunks of 1 KB: half of 16 rows' pieces
+  static_assert(CHUNKS % WAVES == 0 && WM % 64 == 0 && BN % WN == 0 && 128 % WN == 0, "tile shape");
+  constexpr int SCALES = kE4M3 ? WAVES * WM * 4 : 0;                          // each wave's own
+  constexpr int STAGE = CHUNKS * 1024 + SCALES;
+  __shared__ __align__(1024) char lds[2][STAGE];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+  // tiles in bands of an XCD each, four rows of tiles deep: what runs on an XCD at a time shares its operands there
+  const int total = count_tiles<BM>(offsets, experts, p.rows) * ntiles;
+  const int band = (total + 7) / 8, at = blockIdx.x / 8;
+  const int id = (blockIdx.x % 8) * band + at;
+  if (at >= band || id >= total) return;
+  constexpr int GM = 4;
+  const int mtiles = total / ntiles, group = id / (GM * ntiles), in = id - group * GM * ntiles;
+  const int deep = mtiles - group * GM < GM ? mtiles - group * GM : GM;
+  RowTile tile;
+  if (!find_tile<BM>(offsets, experts, p.rows, group * GM + in % deep, tile)) return;
+  const int64_t n0 = (int64_t)(in / deep) * BN;
+  const int wm = (wave % (BM / WM)) * WM, wn = (wave / (BM / WM)) * WN;
+  const int e = tile.expert < 0 ? 0 : tile.expert;
+  const int kb = (int)((p.k + kBlock - 1) / kBlock);
+  // whole steps
+  const int steps = __builtin_amdgcn_readfirstlane(tile.expert < 0 ? 0 : kE4M3 ? kb : (int)(p.k / STEP));
+
+  const char* xb = uniform(static_cast<const char*>(p.x) + tile.lo * p.x_stride * ES);
+  const char* wb = uniform(static_cast<const char*>(p.w) + (e * p.w_expert_stride + n0 * p.w_stride) * ES);
+  const int xlast = (int)(tile.hi - tile.lo) - 1, wlast = (int)(p.n - n0 < BN ? p.n - n0 : BN) - 1;
+  unsigned off[CH];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int c = wave * CH + i;
+    int row = (c < XC ? c : c - XC) * 8 + (lane >> 3);
+    const int last = c < XC ? xlast : wlast;
+    row = row < last ? row : last;                   // rows past the end: the last one again, whose results are not stored
+    off[i] = (unsigned)(row * (c < XC ? p.x_stride : p.w_stride) * ES) + ((lane ^ (lane >> 3)) & 7) * 16;
+  }
+  const char* sxb = nullptr;
+  unsigned soff[WM / 64];
+  if constexpr (kE4M3) {
+    sxb = uniform(reinterpret_cast<const char*>(p.x_scales + tile.lo));
+#pragma unroll
+    for (int i = 0; i < WM / 64; ++i) {
+      const int row = wm + i * 64 + lane;
+      soff[i] = (unsigned)(row < xlast ? row : xlast) * 4;
+    }
+  }
+  const float* sw = nullptr;
+  if constexpr (kE4M3) sw = p.w_scales + ((int64_t)e * ((p.n + kBlock - 1) / kBlock) + (n0 + wn < p.n ? n0 + wn : p.n - 1) / kBlock) * kb;
+
+  const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)&lds[0][0];
+  auto load = [&](int s) {
+    const unsigned to = lds0 + (s & 1) * STAGE;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int c = wave * CH + i;
+      dma16(to + c * 1024, (c < XC ? xb : wb) + (int64_t)s * kStepBytes, off[i], s, steps);
+    }
+    if constexpr (kE4M3) {
+#pragma unroll
+      for (int i = 0; i < WM / 64; ++i)
+        dma4(to + CHUNKS * 1024 + (wave * WM + i * 64) * 4, sxb + (int64_t)s * p.x_scales_stride * 4, soff[i], s, steps);
+    }
+  };
+
+  f4 acc[MT][NT] = {};
+  constexpr int LOADS = CH + (kE4M3 ? WM / 64 : 0);
+  constexpr int XR = MT < 4 ? MT : 4;                // fragments of x held at a time
+  const int at0 = (lane & 15) * 128 + (((lane >> 4) ^ lane) & 7) * 16;
+  const int at1 = at0 ^ 64;
+  auto step = [&](int s, float sws, auto&& next) {
+    const char* base = lds[s & 1];
+    auto frag = [&](int tile16) {
+      return Frag{*reinterpret_cast<const i4*>(base + at0 + tile16 * 2048), *reinterpret_cast<const i4*>(base + at1 + tile16 * 2048)};
+    };
+    Frag w[NT], x[XR];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) w[j] = frag(XC / 2 + wn / 16 + j);
+#pragma unroll
+    for (int i = 0; i < XR; ++i) x[i] = frag(wm / 16 + i);
+    f4 part[2][NT];
+    float sc[MT];
+    if constexpr (kE4M3) {
+      const float* sx = reinterpret_cast<const float*>(base + CHUNKS * 1024) + wave * WM + (lane & 15);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) sc[i] = sx[i * 16] * sws;
+    }
+    auto add = [&](int i) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(part[i & 1][j][r], sc[i], acc[i][j][r]);
+    };
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        if constexpr (!kE4M3) acc[i][j] = step_16bit<TYPE>(w[j], x[i % XR], acc[i][j]);
+        else part[i & 1][j] = EXACT ? step_e4m3_exact(w[j], x[i % XR]) : step_e4m3(w[j], x[i % XR]);
+      }
+      if (i + XR < MT) x[i % XR] = frag(wm / 16 + i + XR);
+      if constexpr (kE4M3) {
+        if (i > 0) add(i - 1);
+      }
+      if (i == (MT == XR ? 0 : MT - XR + 1)) {       // every fragment has been read: its place may be filled again
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        next();
+      }
+      if constexpr (kE4M3 && !EXACT) {               // each matrix instruction hides the FMAs of an earlier one
+        if (i > 0) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
+          }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (kE4M3) add(MT - 1);
+  };
+  load(0);
+  load(1);
+  float swv = 0.f;
+  for (int s = 0; s < steps; ++s) {
+    float sws = 0.f;
+    if constexpr (kE4M3) {
+      if ((s & 63) == 0) {
+        swv = s + lane < kb ? sw[s + lane] : 0.f;
+        asm volatile("" : "+v"(swv));                // waits here, not where both paths meet
+      }
+      sws = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, swv), s & 63));
+    }
+    // step s has landed; step s + 1 may be under way
+    if (s + 1 < steps) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LOADS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    step(s, sws, [&] { load(s + 2); });
+  }
+  if constexpr (!kE4M3) {
+    const int left = (int)(p.k - (int64_t)steps * STEP);
+    if (tile.expert >= 0 && left > 0) {              // the columns after the last whole step; pieces past the end are zero
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int c = wave * CH + i, piece = (lane ^ (lane >> 3)) & 7;
+        const char* a = (c < XC ? xb : wb) + (int64_t)steps * kStepBytes + off[i];
+        dma16_from(lds0 + (steps & 1) * STAGE + c * 1024, piece * 8 < left ? a : reinterpret_cast<const char*>(zero_piece));
+      }
+      barrier_with_loads();
+      step(steps, 0.f, [] {});
+    }
+  }
+  const float* bias = p.bias && tile.expert >= 0 ? p.bias + (int64_t)e * p.n : nullptr;
+  if (bias || p.slope != 1.f) store_tile<OUT, true, MT, NT>(p, tile.lo + wm, tile.hi, n0 + wn, bias, acc);
+  else store_tile<OUT, false, MT, NT>(p, tile.lo + wm, tile.hi, n0 + wn, bias, acc);
+}
+
+template <int TYPE, int OUT, int BM, int BN, int WM, int WN>
+hipError_t launch(const aeisu_product& p, const int32_t* offsets, int experts, hipStream_t stream) {
+  const int64_t ntiles = (p.n + BN - 1) / BN;
+  const int64_t blocks = (most_tiles(p.rows, experts, offsets != nullptr, BM) * ntiles + 7) / 8 * 8;
+  if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+  product_tiles_kernel<TYPE, OUT, BM, BN, WM, WN>
+      <<<(unsigned)blocks, 64 * (BM / WM) * (BN / WN), 0, stream>>>(p, offsets, experts, (int)ntiles);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_product_128(const aeisu_product& p, const int32_t* offsets, int experts, hipStream_t stream) {
+  return for_types<true>(p, [&](auto type, auto out) { return launch<type(), out(), 128, 128, 64, 64>(p, offsets, experts, stream); });
+}
+
+}  // namespace aeisu

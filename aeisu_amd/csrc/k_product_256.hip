@@ -1,0 +1,225 @@
+// Products in tiles of 256 x 256: eight waves of 128 x 64, two groups that multiply and read in turn.
+#include "product.hpp"
+
+namespace aeisu {
+namespace {
+
+template <int TYPE, int OUT>
+__global__ __launch_bounds__(512, 2) void product_phased_kernel(aeisu_product p, const int32_t* offsets, int experts, int ntiles) {
+  constexpr bool kE4M3 = TYPE == AEISU_TYPE_E4M3;
+  constexpr int ES = kE4M3 ? 1 : 2, STEP = kStepBytes / ES, B = 256, XR = 4, NT = 4, MT = 8;
+  constexpr int XBYTES = B * kStepBytes, SCALES = kE4M3 ? 8 * 128 * 4 : 0;
+  constexpr int STAGE = 2 * XBYTES + SCALES;          // x, w, each wave's scales of its 128 rows
+  constexpr int XL = 4 + (kE4M3 ? 2 : 0), WL = 4;     // a wave's loads of a step: its group's rows of x (and scales); w
+  __shared__ __align__(1024) char lds[2][STAGE];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = wave >> 2, wm = group * 128, wn = (wave & 3) * 64;
+  const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)&lds[0][0];
+  const int kb = (int)((p.k + kBlock - 1) / kBlock), nb = (int)((p.n + kBlock - 1) / kBlock);
+
+  const int total = count_tiles<B>(offsets, experts, p.rows) * ntiles;
+  const int band = (total + 7) / 8, mtiles = total / ntiles;
+
+  struct Tile {
+    RowTile r;
+    int64_t n0;
+    const char *x, *w, *sx = nullptr;
+    const float* sw = nullptr;
+    int steps;
+  } t;
+  unsigned xoff[4], woff[4], soff[2];
+  auto find = [&](int at) {
+    const int id = (blockIdx.x % 8) * band + at;
+    if (at >= band || id >= total) return false;
+    constexpr int GM = 4;
+    const int g = id / (GM * ntiles), in = id - g * GM * ntiles;
+    const int deep = mtiles - g * GM < GM ? mtiles - g * GM : GM;
+    if (!find_tile<B>(offsets, experts, p.rows, g * GM + in % deep, t.r)) return false;
+    t.n0 = (int64_t)(in / deep) * B;
+    const int e = t.r.expert < 0 ? 0 : t.r.expert;
+    t.steps = __builtin_amdgcn_readfirstlane(t.r.expert < 0 ? 0 : kE4M3 ? kb : (int)(p.k / STEP));
+    t.x = uniform(static_cast<const char*>(p.x) + t.r.lo * p.x_stride * ES);
+    t.w = uniform(static_cast<const char*>(p.w) + (e * p.w_expert_stride + t.n0 * p.w_stride) * ES);
+    const int xlast = (int)(t.r.hi - t.r.lo) - 1, wlast = (int)(p.n - t.n0 < B ? p.n - t.n0 : B) - 1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {                     // rows past the end: the last one again, whose results are not stored
+      const int xr = wm + (wave & 3) * 32 + i * 8 + (lane >> 3), wr = wave * 32 + i * 8 + (lane >> 3);
+      const unsigned piece = ((lane ^ (lane >> 3)) & 7) * 16;
+      xoff[i] = (unsigned)((xr < xlast ? xr : xlast) * p.x_stride * ES) + piece;
+      woff[i] = (unsigned)((wr < wlast ? wr : wlast) * p.w_stride * ES) + piece;
+    }
+    if constexpr (kE4M3) {
+      t.sx = uniform(reinterpret_cast<const char*>(p.x_scales + t.r.lo));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = wm + i * 64 + lane;
+        soff[i] = (unsigned)(row < xlast ? row : xlast) * 4;
+      }
+      const int64_t wrow = t.n0 + wn < p.n ? t.n0 + wn : p.n - 1;
+      t.sw = p.w_scales + ((int64_t)e * nb + wrow / kBlock) * kb;
+    }
+    return true;
+  };
+  auto load_x = [&](int s) {
+    const unsigned to = lds0 + (s & 1) * STAGE;
+    dma16x4(to + (wm + (wave & 3) * 32) * kStepBytes, t.x + (int64_t)s * kStepBytes, xoff, s, t.steps);
+    if constexpr (kE4M3)
+      dma4x2(to + 2 * XBYTES + wave * 128 * 4, t.sx + (int64_t)s * p.x_scales_stride * 4, soff, s, t.steps);
+  };
+  auto load_w = [&](int s) {
+    dma16x4(lds0 + (s & 1) * STAGE + XBYTES + wave * 32 * kStepBytes, t.w + (int64_t)s * kStepBytes, woff, s, t.steps);
+  };
+  auto preload = [&] {
+    load_w(0);
+    load_x(0);
+    load_w(1);
+    load_x(1);
+  };
+
+  const int at0 = (lane & 15) * kStepBytes + (((lane >> 4) ^ lane) & 7) * 16, at1 = at0 ^ 64;
+  f4 acc[MT][NT];
+  constexpr int HALF = 4 * NT, LAG = 3;               // products of half a step; a product's sum is scaled three later
+  f4 part[LAG + 1];
+  Frag w[NT], x[XR];
+  float sc[4];                                        // scales of the half's rows
+  auto add = [&](int half, int q) {                   // product q of the half
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      acc[half * 4 + q / NT][q % NT][r] = __builtin_fmaf(part[q & LAG][r], sc[q / NT], acc[half * 4 + q / NT][q % NT][r]);
+  };
+  auto frag = [&](const char* base, int row) {
+    return Frag{*reinterpret_cast<const i4*>(base + at0 + row * kStepBytes), *reinterpret_cast<const i4*>(base + at1 + row * kStepBytes)};
+  };
+  // half of a step's products: 64 of the wave's rows
+  auto multiply = [&](int half) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int q = 0; q < HALF; ++q) {
+      const int i = q / NT, j = q % NT;
+      if constexpr (!kE4M3) acc[half * 4 + i][j] = step_16bit<TYPE>(w[j], x[i], acc[half * 4 + i][j]);
+      else {
+        part[q & LAG] = step_e4m3(w[j], x[i]);
+        if (q >= LAG) add(half, q - LAG);
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
+      }
+      if (j == NT - 1) __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto finish = [&](int half) {                       // the half's last sums
+#pragma unroll
+    for (int q = HALF - LAG; q < HALF; ++q) add(half, q);
+  };
+  auto read = [&](int s, int half) {
+    const char* base = lds[s & 1];
+    if (half == 0) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) w[j] = frag(base + XBYTES, wn + j * 16);
+    }
+#pragma unroll
+    for (int i = 0; i < XR; ++i) x[i] = frag(base, wm + half * 64 + i * 16);
+  };
+  auto scales = [&](int s, int half, float sws) {
+    const float* sx = reinterpret_cast<const float*>(lds[s & 1] + 2 * XBYTES) + wave * 128 + half * 64 + (lane & 15);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sc[i] = sx[i * 16] * sws;
+  };
+
+  int at = blockIdx.x / 8;
+  if (!find(at)) return;
+  preload();
+  for (;;) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j <= LAG; ++j) part[j] = f4{0.f, 0.f, 0.f, 0.f};
+    float swv = 0.f;
+    sc[3] = 0.f;
+    barrier_with_loads();
+    if (group == 1) asm volatile("s_barrier" ::: "memory");
+    for (int s = 0; s < t.steps; ++s) {
+      float sws = 0.f;
+      if constexpr (kE4M3) {
+        if ((s & 63) == 0) {
+          swv = s + lane < kb ? t.sw[s + lane] : 0.f;
+          asm volatile("" : "+v"(swv));               // waits here, not where both paths meet
+        }
+        sws = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, swv), s & 63));
+      }
+      read(s, 0);
+      if (s > 0) load_x(s + 1);
+      if constexpr (kE4M3) {
+        finish(1);
+        scales(s, 0, sws);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      multiply(0);
+      asm volatile("s_barrier" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      read(s, 1);
+      load_w(s + 2);
+      if constexpr (kE4M3) {
+        finish(0);
+        scales(s, 1, sws);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      barrier_behind<XL + WL>(s + 2, t.steps);
+      multiply(1);
+      barrier_behind<WL>(s + 2, t.steps);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (kE4M3) finish(1);
+    if (group == 0) asm volatile("s_barrier" ::: "memory");
+    if constexpr (!kE4M3) {
+      const int left = (int)(p.k - (int64_t)(p.k / STEP) * STEP);
+      if (t.r.expert >= 0 && left > 0) {              // the columns after the last whole step; pieces past the end are zero
+        const int s = t.steps, piece = ((lane ^ (lane >> 3)) & 7) * 8;
+        const unsigned to = lds0 + (s & 1) * STAGE;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const char* xa = t.x + (int64_t)s * kStepBytes + xoff[i];
+          const char* wa = t.w + (int64_t)s * kStepBytes + woff[i];
+          dma16_from(to + (wm + (wave & 3) * 32 + i * 8) * kStepBytes, piece < left ? xa : reinterpret_cast<const char*>(zero_piece));
+          dma16_from(to + XBYTES + (wave * 32 + i * 8) * kStepBytes, piece < left ? wa : reinterpret_cast<const char*>(zero_piece));
+        }
+        barrier_with_loads();
+        read(s, 0);
+        multiply(0);
+        read(s, 1);
+        multiply(1);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      }
+    }
+    // the next tile's first steps come in while this one is stored
+    const int64_t m0 = t.r.lo + wm, end = t.r.hi, n0 = t.n0 + wn;
+    const bool any = t.r.expert >= 0;
+    const float* bias = p.bias && any ? p.bias + (int64_t)t.r.expert * p.n : nullptr;
+    at += gridDim.x / 8;
+    const bool more = find(at);
+    if (more) preload();
+    if (bias || p.slope != 1.f) store_tile<OUT, true, MT, NT>(p, m0, end, n0, bias, acc);
+    else store_tile<OUT, false, MT, NT>(p, m0, end, n0, bias, acc);
+    if (!more) return;
+  }
+}
+
+template <int TYPE, int OUT>
+hipError_t launch(const aeisu_product& p, const int32_t* offsets, int experts, int cus, hipStream_t stream) {
+  const int64_t ntiles = (p.n + 255) / 256;
+  int64_t blocks = (most_tiles(p.rows, experts, offsets != nullptr, 256) * ntiles + 7) / 8 * 8;
+  if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+  if (blocks > cus) blocks = cus / 8 * 8;            // each stays on a CU and takes tile after tile
+  product_phased_kernel<TYPE, OUT><<<(unsigned)blocks, 512, 0, stream>>>(p, offsets, experts, (int)ntiles);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_product_256(const aeisu_product& p, const int32_t* offsets, int experts, int cus, hipStream_t stream) {
+  return for_types<false>(p, [&](auto type, auto out) { return launch<type(), out()>(p, offsets, experts, cus, stream); });
+}
+
+}  // namespace aeisu

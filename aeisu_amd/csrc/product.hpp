@@ -43,52 +43,70 @@ struct RowTile {
   int expert;
 };
 
-// The t-th tile of at most BM rows.  Every wave finds it by itself: 64 segments at a time, one a lane.  The segments
-// are the rows before the first offset, each expert's and those after the last offset; a running maximum of the
-// offsets, kept within the rows, bounds them, so they cover every row once whatever the offsets hold.
+// One 64-segment window of the rows' division: the segments are the rows before the first offset, each expert's and those
+// after the last offset, one a lane.  A running maximum of the offsets, kept within the rows, bounds them, so they
+// cover every row once whatever the offsets hold.
 template <int BM>
-__device__ __forceinline__ bool find_tile(const int32_t* offsets, int experts, int64_t rows, int64_t t, RowTile& out) {
-  if (!offsets) {
-    out.lo = t * BM;
-    out.hi = out.lo + BM < rows ? out.lo + BM : rows;
-    out.expert = 0;
-    return out.lo < rows;
-  }
-  const int lane = lane_id(), m = (int)rows;
-  int before = 0;                                    // the previous segments' end
-  int64_t first = 0;                                 // and their tiles
-  for (int s0 = 0; s0 < experts + 2; s0 += 64) {
-    const int s = s0 + lane;                         // segment s ends at offsets[s]; the last one at `rows`
-    int end = s <= experts ? offsets[s] : m;
-    end = end < 0 ? 0 : end > m ? m : end;
+struct Segments {
+  int begin, end, tiles, sum;                        // this lane's rows and tiles; tiles up to and with it
+  __device__ __forceinline__ Segments(const int32_t* offsets, int experts, int rows, int first_segment, int before) {
+    const int lane = lane_id(), s = first_segment + lane;   // segment s ends at offsets[s]; the last one at `rows`
+    end = s <= experts ? offsets[s] : rows;
+    end = end < 0 ? 0 : end > rows ? rows : end;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int o = __shfl_up(end, d);
       if (lane >= d) end = end > o ? end : o;
     }
     end = end > before ? end : before;
-    int begin = __shfl_up(end, 1);
+    begin = __shfl_up(end, 1);
     if (lane == 0) begin = before;
-    const int tiles = (end - begin + BM - 1) / BM;
-    int sum = tiles;                                 // inclusive
+    sum = tiles = (end - begin + BM - 1) / BM;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int o = __shfl_up(sum, d);
       if (lane >= d) sum += o;
     }
-    const uint64_t past = __ballot(first + sum > t);
+  }
+};
+
+// Number of tiles of at most BM rows.
+template <int BM>
+__device__ __forceinline__ int count_tiles(const int32_t* offsets, int experts, int64_t rows) {
+  if (!offsets) return (int)((rows + BM - 1) / BM);
+  int total = 0, before = 0;
+  for (int s0 = 0; s0 < experts + 2; s0 += 64) {
+    const Segments<BM> g(offsets, experts, (int)rows, s0, before);
+    total += __builtin_amdgcn_readlane(g.sum, 63);
+    before = __builtin_amdgcn_readlane(g.end, 63);
+  }
+  return total;
+}
+
+// The t-th tile; every wave finds it by itself.
+template <int BM>
+__device__ __forceinline__ bool find_tile(const int32_t* offsets, int experts, int64_t rows, int t, RowTile& out) {
+  if (!offsets) {
+    out.lo = (int64_t)t * BM;
+    out.hi = out.lo + BM < rows ? out.lo + BM : rows;
+    out.expert = 0;
+    return out.lo < rows;
+  }
+  int first = 0, before = 0;                         // tiles and end of the windows before
+  for (int s0 = 0; s0 < experts + 2; s0 += 64) {
+    const Segments<BM> g(offsets, experts, (int)rows, s0, before);
+    const uint64_t past = __ballot(first + g.sum > t);
     if (past) {
-      const int l = __builtin_ctzll(past);
-      const int64_t at = __shfl(begin, l) + (t - first - (__shfl(sum, l) - __shfl(tiles, l))) * BM;
-      const int64_t e = __shfl(end, l);
-      const int seg = s0 + l;
-      out.lo = at;
-      out.hi = at + BM < e ? at + BM : e;
+      const int l = __builtin_ctzll(past), seg = s0 + l;
+      const int begin = __builtin_amdgcn_readlane(g.begin, l), end = __builtin_amdgcn_readlane(g.end, l);
+      const int in = t - first - (__builtin_amdgcn_readlane(g.sum, l) - __builtin_amdgcn_readlane(g.tiles, l));
+      out.lo = begin + (int64_t)in * BM;
+      out.hi = out.lo + BM < end ? out.lo + BM : end;
       out.expert = seg >= 1 && seg <= experts ? seg - 1 : -1;
       return true;
     }
-    first += __shfl(sum, 63);
-    before = __shfl(end, 63);
+    first += __builtin_amdgcn_readlane(g.sum, 63);
+    before = __builtin_amdgcn_readlane(g.end, 63);
   }
   return false;
 }
@@ -98,6 +116,73 @@ inline int64_t most_tiles(int64_t rows, int experts, bool grouped, int bm) {
   if (!grouped) return (rows + bm - 1) / bm;
   const int64_t t = rows / bm + experts + 2;
   return t < rows ? t : rows;
+}
+
+// ---- tiles through LDS ----------------------------------------------------------------------------------
+// Operands go from memory to LDS without passing through registers: each instruction moves 64 pieces of 16 bytes, one
+// for each lane from an address of its own to 1 KB of adjacent LDS, in the order in which a fragment is read back.
+// The compiler does not see these loads: the barriers below wait for them.  m0 (the LDS address) has no other use here;
+// it settles in one state, and a scalar register that a vector instruction wrote may be read by a load five states
+// later, which is what precedes each first load.
+// Nothing is issued for a step past the last one (a branch that the compiler does not see, so it may schedule across).
+__device__ __forceinline__ void dma16(unsigned lds, const void* base, unsigned offset, int step, int steps) {
+  asm volatile("s_cmp_ge_i32 %3, %4\n\ts_cbranch_scc1 1f\n\ts_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, %2\n1:"
+               ::"s"(lds), "v"(offset), "s"(base), "s"(step), "s"(steps) : "memory", "scc");
+}
+__device__ __forceinline__ void dma4(unsigned lds, const void* base, unsigned offset, int step, int steps) {
+  asm volatile("s_cmp_ge_i32 %3, %4\n\ts_cbranch_scc1 1f\n\ts_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dword %1, %2\n1:"
+               ::"s"(lds), "v"(offset), "s"(base), "s"(step), "s"(steps) : "memory", "scc");
+}
+// Four of them to 4 KB of LDS, and two of 4 bytes a lane to 512 bytes
+__device__ __forceinline__ void dma16x4(unsigned lds, const void* base, const unsigned (&offset)[4], int step, int steps) {
+  asm volatile(
+      "s_cmp_ge_i32 %6, %7\n\ts_cbranch_scc1 1f\n\t"
+      "s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, %5\n\t"
+      "s_add_u32 m0, %0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %5\n\t"
+      "s_add_u32 m0, %0, 0x800\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %5\n\t"
+      "s_add_u32 m0, %0, 0xc00\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %5\n1:"
+      ::"s"(lds), "v"(offset[0]), "v"(offset[1]), "v"(offset[2]), "v"(offset[3]), "s"(base), "s"(step), "s"(steps)
+      : "memory", "scc");
+}
+__device__ __forceinline__ void dma4x2(unsigned lds, const void* base, const unsigned (&offset)[2], int step, int steps) {
+  asm volatile(
+      "s_cmp_ge_i32 %4, %5\n\ts_cbranch_scc1 1f\n\t"
+      "s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dword %1, %3\n\t"
+      "s_add_u32 m0, %0, 0x100\n\ts_nop 0\n\tglobal_load_lds_dword %2, %3\n1:"
+      ::"s"(lds), "v"(offset[0]), "v"(offset[1]), "s"(base), "s"(step), "s"(steps) : "memory", "scc");
+}
+// Barrier for a wave whose loads but the youngest N have landed; for all of them when there is no step `step`, whose
+// loads would be the youngest.
+template <int N>
+__device__ __forceinline__ void barrier_behind(int step, int steps) {
+  asm volatile("s_cmp_lt_i32 %1, %2\n\ts_cbranch_scc1 1f\n\ts_waitcnt vmcnt(0)\n1:\ts_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier"
+               ::"n"(N), "s"(step), "s"(steps) : "memory", "scc");
+}
+__device__ __forceinline__ void dma16_from(unsigned lds, const void* address) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(address) : "memory");
+}
+__device__ __forceinline__ void barrier_with_loads() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+__device__ __forceinline__ f4 step_e4m3(const Frag& w, const Frag& x) {
+  union { i4 h[2]; i8v v; } a{{w.lo, w.hi}}, b{{x.lo, x.hi}};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.v, b.v, f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ const char* uniform(const char* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v), hi = __builtin_amdgcn_readfirstlane((unsigned)(v >> 32));
+  return reinterpret_cast<const char*>(lo | (uint64_t)hi << 32);   // via unsigned: the builtin's int would extend its sign
+}
+// sixteen bytes of zeros, for pieces of a row past its end
+static __device__ __align__(16) const unsigned zero_piece[4] = {0, 0, 0, 0};
+
+// Two results in 16 bits each, to nearest even
+template <int OUT>
+__device__ __forceinline__ unsigned pack16(float a, float b) {
+  if constexpr (OUT == AEISU_TYPE_F16) return pack_h2(a, b);
+  typedef float f2v __attribute__((ext_vector_type(2)));
+  typedef __bf16 b2v __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, __builtin_convertvector((f2v){a, b}, b2v));
 }
 
 // Four results of row m from column n on: bias, activation, one rounding to the result's type.
@@ -128,5 +213,87 @@ __device__ __forceinline__ void finish4(const aeisu_product& p, int64_t m, int64
   else
     for (int i = 0; i < 4 && i < left; ++i) o[i] = b[i];
 }
+
+// Results of a wave's MT x NT accumulators, rows m0 + 16 i + (lane & 15) below `end`, columns n0 + 16 j + 4 (lane >> 4) + r:
+// bias, activation, one rounding to the result's type.  16-bit results of two adjacent accumulators are exchanged
+// between lanes so that each lane stores eight adjacent ones.
+template <int OUT, bool ACT, int MT, int NT>
+__device__ __forceinline__ void store_tile(const aeisu_product& p, int64_t m0, int64_t end, int64_t n0, const float* bias, f4 (&acc)[MT][NT]) {
+  const int lane = lane_id(), g = lane >> 4;
+  constexpr int OS = OUT == AEISU_TYPE_F32 ? 4 : 2;
+  if constexpr (ACT) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      f4 b = {0.f, 0.f, 0.f, 0.f};
+      if (bias) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int64_t n = n0 + j * 16 + 4 * g + r;
+          b[r] = bias[n < p.n ? n : p.n - 1];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float v = acc[i][j][r] + b[r];
+          acc[i][j][r] = v < 0.f ? (p.slope > 0.f ? v * p.slope : 0.f) : v;
+        }
+    }
+  }
+  int64_t m = m0 + (lane & 15);
+  char* row = static_cast<char*>(p.out) + m * p.out_stride * OS;
+#pragma unroll
+  for (int i = 0; i < MT; ++i, m += 16, row += 16 * OS * p.out_stride) {
+    if constexpr (OUT == AEISU_TYPE_F32) {
+      if (m >= end) continue;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int64_t n = n0 + j * 16 + 4 * g, left = p.n - n;
+        float* o = reinterpret_cast<float*>(row) + n;
+        if (left >= 4) __builtin_memcpy(o, &acc[i][j], 16);
+        else
+          for (int r = 0; r < 4; ++r)
+            if (r < left) o[r] = acc[i][j][r];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NT; j += 2) {
+        unsigned a[2], b[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          a[r] = pack16<OUT>(acc[i][j][2 * r], acc[i][j][2 * r + 1]);
+          b[r] = pack16<OUT>(acc[i][j + 1][2 * r], acc[i][j + 1][2 * r + 1]);
+          permlane16_swap_u(a[r], b[r]);             // lane rows 0, 2: the first accumulator's, 1, 3: the second's
+        }
+        const unsigned v[4] = {a[0], a[1], b[0], b[1]};
+        const int64_t n = n0 + (j + (g & 1)) * 16 + 8 * (g >> 1), left = m < end ? p.n - n : 0;
+        unsigned short* o = reinterpret_cast<unsigned short*>(row) + n;
+        if (left >= 8) __builtin_memcpy(o, v, 16);
+        else
+          for (int r = 0; r < 8; ++r)
+            if (r < left) o[r] = (unsigned short)(v[r >> 1] >> 16 * (r & 1));
+      }
+    }
+  }
+}
+
+// fn<type, result type>: a launch for each pair of them; E4M3 with FP32 results where the kernel has it
+template <bool EXACT, typename Fn>
+hipError_t for_types(const aeisu_product& p, Fn fn) {
+  auto out = [&](auto type) {
+    if (p.out_type == AEISU_TYPE_F16) return fn(type, std::integral_constant<int, AEISU_TYPE_F16>());
+    if (p.out_type == AEISU_TYPE_BF16) return fn(type, std::integral_constant<int, AEISU_TYPE_BF16>());
+    if constexpr (EXACT || type() != AEISU_TYPE_E4M3) return fn(type, std::integral_constant<int, AEISU_TYPE_F32>());
+    return hipErrorInvalidValue;
+  };
+  if (p.type == AEISU_TYPE_E4M3) return out(std::integral_constant<int, AEISU_TYPE_E4M3>());
+  if (p.type == AEISU_TYPE_F16) return out(std::integral_constant<int, AEISU_TYPE_F16>());
+  return out(std::integral_constant<int, AEISU_TYPE_BF16>());
+}
+
+hipError_t launch_product_256(const aeisu_product& p, const int32_t* offsets, int experts, int cus, hipStream_t stream);
+hipError_t launch_product_128(const aeisu_product& p, const int32_t* offsets, int experts, hipStream_t stream);
+hipError_t launch_product_rows(const aeisu_product& p, const int32_t* offsets, int experts, int mt, int nt, hipStream_t stream);
 
 }  // namespace aeisu
