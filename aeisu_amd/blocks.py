@@ -15,7 +15,7 @@ that cannot be served raise ``ValueError``.  The HIP kernels of ``libaeisu_amd.s
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 from typing import Optional, Union
 
 import torch
@@ -30,11 +30,6 @@ def _blocks(n: int) -> int:
     return -(-n // BLOCK)
 
 
-def _require(ok: bool, message: str) -> None:
-    if not ok:
-        raise ValueError(message)
-
-
 class QuantRows:
     """E4M3 rows: value[r, c] = codes[r, c] * scales[c // 128, r].
 
@@ -45,12 +40,14 @@ class QuantRows:
     __slots__ = ("codes", "scales", "cols")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, cols: int):
-        _require(codes.dtype == torch.uint8 and codes.ndim == 2 and scales.dtype == torch.float32 and scales.ndim == 2,
-                 "codes are uint8 [rows, padded columns], scales float32 [blocks, rows]")
+        if codes.dtype != torch.uint8 or codes.ndim != 2 or scales.dtype != torch.float32:
+            raise ValueError("codes are uint8 [rows, padded columns], scales float32 [blocks, rows]")
         nb = -(-cols // BLOCK)
-        _require(cols >= 0 and codes.shape[1] >= nb * BLOCK and scales.shape == (nb, codes.shape[0]),
-                 f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not hold rows of {cols} columns")
-        _require(codes.device == scales.device, "codes and scales lie on different devices")
+        rows, wide = codes.shape
+        if cols < 0 or wide < nb * BLOCK or scales.shape != (nb, rows):
+            raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not hold rows of {cols} columns")
+        if codes.device != scales.device:
+            raise ValueError("codes and scales lie on different devices")
         self.codes, self.scales, self.cols = codes, scales, cols
 
     @property
@@ -77,13 +74,14 @@ class QuantWeight:
     __slots__ = ("codes", "scales", "cols")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, cols: int):
-        _require(codes.dtype == torch.uint8 and codes.ndim in (2, 3) and scales.dtype == torch.float32,
-                 "codes are uint8 [(experts,) n, padded columns], scales float32")
+        if codes.dtype != torch.uint8 or codes.ndim not in (2, 3) or scales.dtype != torch.float32:
+            raise ValueError("codes are uint8 [(experts,) n, padded columns], scales float32")
         nb = -(-cols // BLOCK)
-        want = (*codes.shape[:-2], -(-codes.shape[-2] // BLOCK), nb)
-        _require(cols >= 0 and codes.shape[-1] >= nb * BLOCK and scales.shape == want and scales.is_contiguous(),
-                 f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not hold rows of {cols} columns")
-        _require(codes.device == scales.device, "codes and scales lie on different devices")
+        *lead, n, wide = codes.shape
+        if cols < 0 or wide < nb * BLOCK or scales.shape != (*lead, -(-n // BLOCK), nb) or not scales.is_contiguous():
+            raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not hold rows of {cols} columns")
+        if codes.device != scales.device:
+            raise ValueError("codes and scales lie on different devices")
         self.codes, self.scales, self.cols = codes, scales, cols
 
     @property
@@ -102,15 +100,18 @@ class QuantWeight:
 
 
 # ---- calls ---------------------------------------------------------------------------------------------
+# What a call costs on the host is what small calls cost: messages are made only when they are raised, the current
+# stream and device are asked for without their objects, and the descriptor is packed in one go.
 def _stream(device: torch.device, stream: Optional[torch.cuda.Stream]) -> int:
     if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream
-    _require(stream.device == device, f"the stream belongs to {stream.device}, the tensors to {device}")
+        return torch._C._cuda_getCurrentRawStream(device.index)
+    if stream.device != device:
+        raise ValueError(f"the stream belongs to {stream.device}, the tensors to {device}")
     return stream.cuda_stream
 
 
 def _call(device: torch.device, fn, *args) -> None:
-    if device.index == torch.cuda.current_device():
+    if device.index == torch._C._cuda_getDevice():
         rc = fn(*args)
     else:
         with torch.cuda.device(device):
@@ -120,16 +121,11 @@ def _call(device: torch.device, fn, *args) -> None:
 
 
 def _new(shape, dtype, device, stream) -> torch.Tensor:
-    """A result of a call on ``stream``: its memory may be reused for work on the current stream only, and the
-    other stream's work is not awaited by it."""
+    """A result of a call on ``stream``: told to the allocator where that is not the current one."""
     t = torch.empty(shape, dtype=dtype, device=device)
     if stream is not None:
         t.record_stream(stream)
     return t
-
-
-def _on_device(t: torch.Tensor, device: torch.device, what: str) -> None:
-    _require(t.device == device, f"{what} lies on {t.device}, not on {device}")
 
 
 def quantize_rows(x: torch.Tensor, rows: Optional[torch.Tensor] = None, gated: bool = False,
@@ -142,16 +138,17 @@ def quantize_rows(x: torch.Tensor, rows: Optional[torch.Tensor] = None, gated: b
     its own place.  The columns of ``x`` have to be adjacent, its rows may lie anywhere.
     """
     dtype = _TYPES.get(x.dtype)
-    _require(x.is_cuda and dtype is not None and x.ndim == 2 and (x.stride(1) == 1 or x.shape[1] <= 1),
-             "x is a float16, bfloat16 or float32 matrix on a HIP device with adjacent columns")
+    if dtype is None or not x.is_cuda or x.ndim != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
+        raise ValueError("x is a float16, bfloat16 or float32 matrix on a HIP device with adjacent columns")
     m, k = x.shape
     if gated:
-        _require(k % 2 == 0, "a gated x has two halves of equal width")
+        if k % 2:
+            raise ValueError("a gated x has two halves of equal width")
         k //= 2
     device, n, index = x.device, m, 0
     if rows is not None:
-        _on_device(rows, device, "rows")
-        _require(rows.dtype == torch.int32 and rows.ndim == 1 and rows.is_contiguous(), "rows are contiguous int32 indices")
+        if rows.device != device or rows.dtype != torch.int32 or rows.ndim != 1 or not rows.is_contiguous():
+            raise ValueError("rows are contiguous int32 indices on x's device")
         n, index = rows.shape[0], rows.data_ptr()
     kb = -(-k // BLOCK)
     codes = _new((n, kb * BLOCK), torch.uint8, device, stream)
@@ -166,8 +163,8 @@ def quantize_weight(w: torch.Tensor, stream: Optional[torch.cuda.Stream] = None)
     """[n, k] or [experts, n, k] float16 / bfloat16 / float32 -> E4M3 weights with a scale for each 128 x 128 tile,
     by the rule of ``quantize_rows``."""
     dtype = _TYPES.get(w.dtype)
-    _require(w.is_cuda and dtype is not None and w.ndim in (2, 3) and (w.stride(-1) == 1 or w.shape[-1] <= 1),
-             "w is a float16, bfloat16 or float32 [n, k] or [experts, n, k] on a HIP device with adjacent columns")
+    if dtype is None or not w.is_cuda or w.ndim not in (2, 3) or (w.stride(-1) != 1 and w.shape[-1] > 1):
+        raise ValueError("w is a float16, bfloat16 or float32 [n, k] or [experts, n, k] on a HIP device with adjacent columns")
     n, k = w.shape[-2:]
     e = w.shape[0] if w.ndim == 3 else 1
     lead = w.shape[:-2]
@@ -179,56 +176,64 @@ def quantize_weight(w: torch.Tensor, stream: Optional[torch.cuda.Stream] = None)
     return QuantWeight(codes, scales, k)
 
 
+_descriptor = struct.Struct("@iiqqqPqPqPqqPPfPq")       # aeisu_product
+
+
 def _product(x, w, offsets, bias, slope, out_dtype, out, stream) -> torch.Tensor:
-    grouped = offsets is not None
-    device = x.device
-    if isinstance(x, QuantRows):
-        _require(isinstance(w, QuantWeight), "quantised rows are multiplied by a QuantWeight")
-        kind, xt, wt, k, wk = L.TYPE_E4M3, x.codes, w.codes, x.cols, w.cols
-        x_scales, x_scales_stride, w_scales = x.scales.data_ptr(), x.scales.stride(0), w.scales.data_ptr()
-        _require((x.scales.stride(1) == 1 or x.scales.shape[1] <= 1) and xt.stride(1) == 1 and wt.stride(-1) == 1,
-                 "the columns of codes and the rows of scales have to be adjacent")
+    if type(x) is QuantRows:
+        if type(w) is not QuantWeight:
+            raise ValueError("quantised rows are multiplied by a QuantWeight")
+        kind, xt, wt, k, wk, xs = L.TYPE_E4M3, x.codes, w.codes, x.cols, w.cols, x.scales
+        x_scales, x_scales_stride, w_scales = xs.data_ptr(), xs.stride(0), w.scales.data_ptr()
+        adjacent = xs.stride(1) == 1 or xs.shape[1] <= 1
     else:
-        _require(isinstance(x, torch.Tensor) and isinstance(w, torch.Tensor) and x.dtype == w.dtype
-                 and x.dtype in (torch.float16, torch.bfloat16) and x.ndim == 2,
-                 "x and w are QuantRows and QuantWeight, or float16 / bfloat16 tensors of one type")
+        if not (isinstance(x, torch.Tensor) and isinstance(w, torch.Tensor) and x.dtype == w.dtype
+                and x.dtype in (torch.float16, torch.bfloat16) and x.ndim == 2):
+            raise ValueError("x and w are QuantRows and QuantWeight, or float16 / bfloat16 tensors of one type")
         kind, xt, wt, k, wk = _TYPES[x.dtype], x, w, x.shape[1], w.shape[-1]
         x_scales = x_scales_stride = w_scales = 0
-        _require((x.stride(1) == 1 or k <= 1) and (w.stride(-1) == 1 or wk <= 1), "the columns of x and w have to be adjacent")
-    _require(wt.ndim == (3 if grouped else 2), "w is [experts, n, k]" if grouped else "w is [n, k]")
-    m, n = xt.shape[0], wt.shape[-2]
-    _require(k == wk, f"x has {k} columns, w has {wk}")
-    _require(xt.is_cuda and wt.device == device, "x and w lie on one HIP device")
+        adjacent = True
+    device, m, wshape = xt.device, xt.shape[0], wt.shape
+    if len(wshape) != (2 if offsets is None else 3):
+        raise ValueError("w is [n, k]" if offsets is None else "w is [experts, n, k]")
+    n = wshape[-2]
+    if k != wk:
+        raise ValueError(f"x has {k} columns, w has {wk}")
+    xstride, wstride = xt.stride(), wt.stride()
+    if not adjacent or (xstride[1] != 1 or wstride[-1] != 1) and k > 1:
+        raise ValueError("the columns of x and w, and the rows of x's scales, have to be adjacent")
+    if not xt.is_cuda or wt.device != device:
+        raise ValueError("x and w lie on one HIP device")
     if out is None:
         out_dtype = out_dtype or (torch.float16 if kind == L.TYPE_E4M3 else x.dtype)
-        _require(out_dtype in _TYPES, "results are float16, bfloat16 or float32")
-        out = _new((m, n), out_dtype, device, stream)
+        if out_dtype not in _TYPES:
+            raise ValueError("results are float16, bfloat16 or float32")
+        out, ostride = _new((m, n), out_dtype, device, stream), n
     else:
-        _on_device(out, device, "out")
-        _require(out.shape == (m, n) and out.dtype in _TYPES and out_dtype in (None, out.dtype)
-                 and (out.stride(1) == 1 or n <= 1) and (out.stride(0) >= n or m <= 1),
-                 f"out is a [{m}, {n}] matrix of the result's type with adjacent columns")
-    bp = 0
-    if bias is not None:
-        _on_device(bias, device, "bias")
-        _require(bias.dtype == torch.float32 and bias.shape == wt.shape[:-1] and bias.is_contiguous(),
-                 f"bias is contiguous float32 {tuple(wt.shape[:-1])}")
-        bp = bias.data_ptr()
-    _require(slope is None or 0 <= slope < float("inf"), "slope is a finite number, at least 0")
-    if grouped:
-        _on_device(offsets, device, "offsets")
-        _require(offsets.dtype == torch.int32 and offsets.is_contiguous() and offsets.shape == (wt.shape[0] + 1,),
-                 f"offsets are {wt.shape[0] + 1} contiguous int32 numbers")
-        _require(wt.shape[0] >= 1, "there is at least one expert")
+        ostride = out.stride(0) if out.ndim == 2 else 0
+        if (out.device != device or out.shape != (m, n) or out.dtype not in _TYPES or out_dtype not in (None, out.dtype)
+                or (out.stride(1) != 1 and n > 1) or (ostride < n and m > 1)):
+            raise ValueError(f"out is a [{m}, {n}] matrix of the result's type with adjacent columns on x's device")
+        out_dtype = out.dtype
+    if bias is not None and (bias.device != device or bias.dtype != torch.float32 or bias.shape != wshape[:-1]
+                             or not bias.is_contiguous()):
+        raise ValueError(f"bias is contiguous float32 {tuple(wshape[:-1])} on x's device")
+    if slope is None:
+        slope = 1.0
+    elif not 0 <= slope < float("inf"):
+        raise ValueError("slope is a finite number, at least 0")
+    if offsets is not None and (offsets.device != device or offsets.dtype != torch.int32 or not offsets.is_contiguous()
+                                or offsets.shape != (wshape[0] + 1,) or wshape[0] < 1):
+        raise ValueError(f"offsets are {wshape[0] + 1} contiguous int32 numbers on x's device, of at least one expert")
     if m == 0 or n == 0:
         return out
-    p = L.Product(kind, _TYPES[out.dtype], m, n, k, xt.data_ptr(), xt.stride(0), x_scales, x_scales_stride, wt.data_ptr(),
-                  wt.stride(-2), wt.stride(0) if grouped else 0, w_scales, bp, 1.0 if slope is None else slope,
-                  out.data_ptr(), out.stride(0))
-    if grouped:
-        _call(device, L.lib().aeisu_grouped_matmul, ctypes.byref(p), offsets.data_ptr(), wt.shape[0], _stream(device, stream))
+    p = _descriptor.pack(kind, _TYPES[out_dtype], m, n, k, xt.data_ptr(), xstride[0], x_scales, x_scales_stride, wt.data_ptr(),
+                         wstride[-2], 0 if offsets is None else wstride[0], w_scales, 0 if bias is None else bias.data_ptr(),
+                         slope, out.data_ptr(), ostride)
+    if offsets is None:
+        _call(device, L.lib().aeisu_matmul, p, _stream(device, stream))
     else:
-        _call(device, L.lib().aeisu_matmul, ctypes.byref(p), _stream(device, stream))
+        _call(device, L.lib().aeisu_grouped_matmul, p, offsets.data_ptr(), wshape[0], _stream(device, stream))
     return out
 
 
@@ -239,7 +244,8 @@ def matmul(x: QuantRows, w: QuantWeight, bias: Optional[torch.Tensor] = None, sl
 
     ``bias`` float32 [n]; ``slope``: LeakyReLU of that slope.
     """
-    _require(isinstance(x, QuantRows) and isinstance(w, QuantWeight), "x and w are a QuantRows and a QuantWeight")
+    if type(x) is not QuantRows or type(w) is not QuantWeight:
+        raise ValueError("x and w are a QuantRows and a QuantWeight")
     return _product(x, w, None, bias, slope, out_dtype, out, stream)
 
 
@@ -254,5 +260,6 @@ def grouped_matmul(x: Union[QuantRows, torch.Tensor], w: Union[QuantWeight, torc
     are a ``QuantRows`` and a ``QuantWeight`` [experts, n, k], or float16 / bfloat16 tensors; ``bias`` float32
     [experts, n].  The result has ``out_dtype`` (unless given: ``out``'s, else float16 for E4M3 operands and theirs for others).
     """
-    _require(isinstance(offsets, torch.Tensor), "offsets are an int32 tensor")
+    if not isinstance(offsets, torch.Tensor):
+        raise ValueError("offsets are an int32 tensor")
     return _product(x, w, offsets, bias, slope, out_dtype, out, stream)
