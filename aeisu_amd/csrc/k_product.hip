@@ -166,7 +166,7 @@ Choice choose(const aeisu_product& p, bool grouped, int experts, int cus) {
   const bool pieces = e4m3 || (p.k % 8 == 0 && p.x_stride % 8 == 0 && p.w_stride % 8 == 0 && p.w_expert_stride % 8 == 0 &&
                                (reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w)) % 16 == 0);
   if (pieces && std::max(p.x_stride, p.w_stride) * es <= (int64_t(1) << 32) / 256 - kStepBytes) {
-    offer(5 + steps * (exact ? 0.97 : 0.62) * std::ceil(share(128, 128)), Choice{Choice::k128, 0, 0});
+    offer(5 + steps * (exact ? 0.97 : 0.62) * std::ceil(share(128, 128)), Choice{Choice::k128, 0, 128});
     if (!exact) offer(8 + (steps * 1.55 + 6) * std::ceil(share(256, 256)), Choice{Choice::k256, 0, 0});
   }
   return best;
@@ -179,7 +179,7 @@ hipError_t launch_product(const aeisu_product& p, const int32_t* offsets, int ex
   const Choice c = choose(p, offsets != nullptr, experts, cus);
   switch (c.kernel) {
     case Choice::k256: return launch_product_256(p, offsets, experts, cus, stream);
-    case Choice::k128: return launch_product_128(p, offsets, experts, stream);
+    case Choice::k128: return launch_product_128(p, offsets, experts, c.nt, stream);
     case Choice::kRows: return launch_product_rows(p, offsets, experts, c.mt, c.nt, stream);
     default: return launch_product_any(p, offsets, experts, stream);
   }

@@ -1,4 +1,4 @@
-// Products in tiles of 128 x 128: four waves of 64 x 64, two blocks on a CU.
+// Products in tiles of 128 x 128 (four waves of 64 x 64, two blocks on a CU) or 128 x 64 (64 x 32, three blocks).
 #include "product.hpp"
 
 namespace aeisu {
@@ -14,7 +14,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void product_tiles_k
   static_assert(CHUNKS % WAVES == 0 && WM % 64 == 0 && BN % WN == 0 && 128 % WN == 0, "tile shape");
   constexpr int SCALES = kE4M3 ? WAVES * WM * 4 : 0;                          // each wave's own
   constexpr int STAGE = CHUNKS * 1024 + SCALES;
-  __shared__ __align__(1024) char lds[2][STAGE];
+  extern __shared__ __align__(1024) char lds[];      // two stages, one where there is one step
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
   // tiles in bands of an XCD each, four rows of tiles deep: what runs on an XCD at a time shares its operands there
@@ -59,7 +59,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void product_tiles_k
   const float* sw = nullptr;
   if constexpr (kE4M3) sw = p.w_scales + ((int64_t)e * ((p.n + kBlock - 1) / kBlock) + (n0 + wn < p.n ? n0 + wn : p.n - 1) / kBlock) * kb;
 
-  const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)&lds[0][0];
+  const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
   auto load = [&](int s) {
     const unsigned to = lds0 + (s & 1) * STAGE;
 #pragma unroll
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void product_tiles_k
   const int at0 = (lane & 15) * 128 + (((lane >> 4) ^ lane) & 7) * 16;
   const int at1 = at0 ^ 64;
   auto step = [&](int s, float sws, auto&& next) {
-    const char* base = lds[s & 1];
+    const char* base = lds + (s & 1) * STAGE;
     auto frag = [&](int tile16) {
       return Frag{*reinterpret_cast<const i4*>(base + at0 + tile16 * 2048), *reinterpret_cast<const i4*>(base + at1 + tile16 * 2048)};
     };
@@ -162,8 +162,9 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void product_tiles_k
     }
   }
   const float* bias = p.bias && tile.expert >= 0 ? p.bias + (int64_t)e * p.n : nullptr;
-  if (bias || p.slope != 1.f) store_tile<OUT, true, MT, NT>(p, tile.lo + wm, tile.hi, n0 + wn, bias, acc);
-  else store_tile<OUT, false, MT, NT>(p, tile.lo + wm, tile.hi, n0 + wn, bias, acc);
+  char* stage = lds + wave * 2048;                   // every fragment has been read, by all waves
+  if (bias || p.slope != 1.f) store_tile<OUT, true, MT, NT>(p, tile.lo + wm, tile.hi, n0 + wn, bias, acc, stage);
+  else store_tile<OUT, false, MT, NT>(p, tile.lo + wm, tile.hi, n0 + wn, bias, acc, stage);
 }
 
 template <int TYPE, int OUT, int BM, int BN, int WM, int WN>
@@ -171,15 +172,25 @@ hipError_t launch(const aeisu_product& p, const int32_t* offsets, int experts, h
   const int64_t ntiles = (p.n + BN - 1) / BN;
   const int64_t blocks = (most_tiles(p.rows, experts, offsets != nullptr, BM) * ntiles + 7) / 8 * 8;
   if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+  constexpr int WAVES = (BM / WM) * (BN / WN), STAGE = (BM + BN) * kStepBytes + (TYPE == AEISU_TYPE_E4M3 ? WAVES * WM * 4 : 0);
+  constexpr int STEP = TYPE == AEISU_TYPE_E4M3 ? kStepBytes : kStepBytes / 2;
+  if constexpr (2 * STAGE > 65536) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&product_tiles_kernel<TYPE, OUT, BM, BN, WM, WN>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, 2 * STAGE);
+    if (e != hipSuccess) return e;
+  }
   product_tiles_kernel<TYPE, OUT, BM, BN, WM, WN>
-      <<<(unsigned)blocks, 64 * (BM / WM) * (BN / WN), 0, stream>>>(p, offsets, experts, (int)ntiles);
+      <<<(unsigned)blocks, 64 * WAVES, p.k > STEP ? 2 * STAGE : STAGE, stream>>>(p, offsets, experts, (int)ntiles);
   return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_product_128(const aeisu_product& p, const int32_t* offsets, int experts, hipStream_t stream) {
-  return for_types<true>(p, [&](auto type, auto out) { return launch<type(), out(), 128, 128, 64, 64>(p, offsets, experts, stream); });
+hipError_t launch_product_128(const aeisu_product& p, const int32_t* offsets, int experts, int columns, hipStream_t stream) {
+  return for_types<true>(p, [&](auto type, auto out) {
+    return columns == 64 ? launch<type(), out(), 128, 64, 64, 32>(p, offsets, experts, stream)
+                         : launch<type(), out(), 128, 128, 64, 64>(p, offsets, experts, stream);
+  });
 }
 
 }  // namespace aeisu

@@ -12,6 +12,7 @@ __global__ __launch_bounds__(512, 2) void product_phased_kernel(aeisu_product p,
   constexpr int STAGE = 2 * XBYTES + SCALES;          // x, w, each wave's scales of its 128 rows
   constexpr int XL = 4 + (kE4M3 ? 2 : 0), WL = 4;     // a wave's loads of a step: its group's rows of x (and scales); w
   __shared__ __align__(1024) char lds[2][STAGE];
+  __shared__ __align__(1024) char stage[OUT == AEISU_TYPE_F32 ? 1 : 8][2048];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int group = wave >> 2, wm = group * 128, wn = (wave & 3) * 64;
   const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)&lds[0][0];
@@ -200,8 +201,8 @@ __global__ __launch_bounds__(512, 2) void product_phased_kernel(aeisu_product p,
     at += gridDim.x / 8;
     const bool more = find(at);
     if (more) preload();
-    if (bias || p.slope != 1.f) store_tile<OUT, true, MT, NT>(p, m0, end, n0, bias, acc);
-    else store_tile<OUT, false, MT, NT>(p, m0, end, n0, bias, acc);
+    if (bias || p.slope != 1.f) store_tile<OUT, true, MT, NT>(p, m0, end, n0, bias, acc, stage[OUT == AEISU_TYPE_F32 ? 0 : wave]);
+    else store_tile<OUT, false, MT, NT>(p, m0, end, n0, bias, acc, stage[OUT == AEISU_TYPE_F32 ? 0 : wave]);
     if (!more) return;
   }
 }

@@ -3,15 +3,13 @@
 //   scale = max(m / 448, 2^-126), m = largest finite |y| of the block;   code = E4M3(fl32(y / scale))
 //
 // One pass over the data: sixteen lanes hold a row's block (eight values each), reduce m among themselves and write
-// eight codes each.  A workgroup takes sixteen rows at one block column, so that the block-major scales leave as
-// 64 consecutive bytes.
+// eight codes each.  A workgroup takes sixteen rows (or groups of them) at one block column, so that the block-major
+// scales leave as 64 consecutive bytes.
 #include "blocks.hpp"
 #include "common.hpp"
 
 namespace aeisu {
 namespace {
-
-typedef unsigned short us8 __attribute__((ext_vector_type(8)));
 
 template <int TYPE>
 using elem_t = typename std::conditional<TYPE == AEISU_TYPE_F32, float, unsigned short>::type;
@@ -23,75 +21,133 @@ __device__ __forceinline__ float widen(elem_t<TYPE> v) {
   else return __builtin_bit_cast(float, (unsigned)v << 16);
 }
 
-// Eight values of a row from column c on, zeros past `left` of them.  Rows need only the alignment of an element:
-// the load of eight is one instruction wherever it starts.
 template <int TYPE>
-__device__ __forceinline__ void load8(const elem_t<TYPE>* p, int64_t left, float v[8]) {
+struct Eight {
+  elem_t<TYPE> e[8];
+};
+
+// Eight values of a row, zeros past `left` of them.  Rows need only the alignment of an element: the load of eight is
+// one instruction (FP32: two) wherever it starts.
+template <int TYPE>
+__device__ __forceinline__ Eight<TYPE> load8(const elem_t<TYPE>* p, int64_t left) {
+  Eight<TYPE> r;
   if (left >= 8) {
-    elem_t<TYPE> e[8];
-    __builtin_memcpy(e, p, sizeof(e));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = widen<TYPE>(e[i]);
+    __builtin_memcpy(r.e, p, sizeof(r.e));
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < left ? widen<TYPE>(p[i]) : 0.f;
+    for (int i = 0; i < 8; ++i) r.e[i] = i < left ? p[i] : elem_t<TYPE>(0);
   }
+  return r;
+}
+template <int TYPE>
+__device__ __forceinline__ void widen8(const Eight<TYPE>& r, float v[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = widen<TYPE>(r.e[i]);
 }
 
-// Largest finite magnitude of eight values
+// Largest finite magnitude of eight values.  `bad` becomes NaN where one is not finite (v * 0); only then are they
+// looked at one by one.
 __device__ __forceinline__ float finite_max(const float v[8]) {
-  float m = 0.f;
+  float m = 0.f, bad = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float a = __builtin_fabsf(v[i]);
-    m = a < __builtin_inff() ? __builtin_fmaxf(m, a) : m;     // false for NaN too
+    m = __builtin_fmaxf(m, __builtin_fabsf(v[i]));
+    bad = __builtin_fmaf(v[i], 0.f, bad);
+  }
+  if (bad != bad) {
+    m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float a = __builtin_fabsf(v[i]);
+      m = a < __builtin_inff() ? __builtin_fmaxf(m, a) : m;   // false for NaN too
+    }
   }
   return m;
+}
+// Largest of sixteen adjacent lanes: rotations within a lane row
+template <int BY>
+__device__ __forceinline__ float rotated(float m) {
+  const int i = __builtin_bit_cast(int, m);
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, 0x120 + BY, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float max16(float m) {
+  m = __builtin_fmaxf(m, rotated<8>(m));
+  m = __builtin_fmaxf(m, rotated<4>(m));
+  m = __builtin_fmaxf(m, rotated<2>(m));
+  return __builtin_fmaxf(m, rotated<1>(m));
 }
 
 __device__ __forceinline__ float block_scale(float m) { return __builtin_fmaxf(m / kE4M3Max, 0x1p-126f); }
 
 // Codes of eight values.  |y / scale| <= 448 (1 + 2^-23) for a finite y, which rounds to at most 448, and the
 // conversion gives the NaN code for NaN and infinity: no clamp.
+// The quotients are rounded correctly, without a division each: r = fl(1 / scale), and two corrections
+// q + r (y - q scale) of q = fl(y r).  The first leaves q within a unit in the last place, and from there the second gives
+// the nearest (Markstein's theorem, r being the nearest to 1 / scale and y - q scale exact).  That remainder is exact
+// while |y| 2^-47 is no denormal number: for scale >= 2^-90 wherever the quotient reaches 2^-10, and below that every
+// code is 0.
 __device__ __forceinline__ uint2 encode8(const float v[8], float scale) {
   float q[8];
+  if (__builtin_expect(scale >= 0x1p-90f, 1)) {
+    const float r = 1.f / scale;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) q[i] = v[i] / scale;
-  uint2 r;
+    for (int i = 0; i < 8; ++i) {
+      q[i] = v[i] * r;
+      q[i] = __builtin_fmaf(__builtin_fmaf(-q[i], scale, v[i]), r, q[i]);
+      q[i] = __builtin_fmaf(__builtin_fmaf(-q[i], scale, v[i]), r, q[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = v[i] / scale;
+  }
+  uint2 c;
   int lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
-  r.x = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
+  c.x = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);
-  r.y = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], lo, true);
-  return r;
+  c.y = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], lo, true);
+  return c;
 }
 
-template <int TYPE, bool GATED>
+// SiLU(a) b.  With t = exp(-|a|) the logistic function is 1 / (1 + t) or t / (1 + t): nothing overflows, and 1 + t in [1, 2]
+// suits the reciprocal instruction (one unit in the last place).
+__device__ __forceinline__ float gate(float a, float b) {
+  const float t = expf(-__builtin_fabsf(a));
+  return (a < 0.f ? a * t : a) * __builtin_amdgcn_rcpf(1.f + t) * b;
+}
+
+// CU block columns for each thread, all loads before the first use.
+template <int TYPE, bool GATED, int CU>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeRows q) {
   const int lane = threadIdx.x & 15;
+  const int64_t nb = (q.cols + kBlock - 1) / kBlock;
   const int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
   if (r >= q.rows) return;                           // whole groups of sixteen lanes
-  int64_t src = r;
-  if (q.index) src = q.index[r];
+  const int64_t src = q.index ? q.index[r] : r;
   const bool have = src >= 0 && src < q.x_rows;
   const elem_t<TYPE>* x = static_cast<const elem_t<TYPE>*>(q.x) + (have ? src : 0) * q.x_stride;
-  const int64_t nb = (q.cols + kBlock - 1) / kBlock;
-  for (int64_t j = blockIdx.y; j < nb; j += gridDim.y) {
-    const int64_t c = j * kBlock + lane * 8;
-    const int64_t left = have ? q.cols - c : 0;
-    float v[8];
-    load8<TYPE>(x + c, left, v);
-    if constexpr (GATED) {
-      float b[8];
-      load8<TYPE>(x + q.cols + c, left, b);
+  for (int64_t j0 = (int64_t)blockIdx.y * CU; j0 < nb; j0 += (int64_t)gridDim.y * CU) {
+    Eight<TYPE> a[CU], b[GATED ? CU : 1];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = v[i] / (1.f + expf(-v[i])) * b[i];
+    for (int j = 0; j < CU; ++j) {
+      const int64_t c = (j0 + j) * kBlock + lane * 8, left = have ? q.cols - c : 0;
+      a[j] = load8<TYPE>(x + c, left);
+      if constexpr (GATED) b[j] = load8<TYPE>(x + q.cols + c, left);
     }
-    float m = finite_max(v);
 #pragma unroll
-    for (int d = 1; d < 16; d <<= 1) m = __builtin_fmaxf(m, __shfl_xor(m, d, 16));
-    const float s = block_scale(m);
-    *reinterpret_cast<uint2*>(q.codes + r * q.codes_stride + c) = encode8(v, s);
-    if (lane == 0) q.scales[j * q.scales_stride + r] = s;
+    for (int j = 0; j < CU; ++j) {
+      if (j0 + j >= nb) break;
+      float v[8];
+      widen8<TYPE>(a[j], v);
+      if constexpr (GATED) {
+        float u[8];
+        widen8<TYPE>(b[j], u);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = gate(v[k], u[k]);
+      }
+      const float s = block_scale(max16(finite_max(v)));
+      *reinterpret_cast<uint2*>(q.codes + r * q.codes_stride + (j0 + j) * kBlock + lane * 8) = encode8(v, s);
+      if (lane == 0) q.scales[(j0 + j) * q.scales_stride + r] = s;
+    }
   }
 }
 
@@ -108,7 +164,7 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(QuantizeWeight q) 
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int64_t r = jn * kBlock + i * 16 + row;
-    load8<TYPE>(w + (r < q.n ? r : 0) * q.row_stride + c, r < q.n ? q.k - c : 0, v[i]);
+    widen8<TYPE>(load8<TYPE>(w + (r < q.n ? r : 0) * q.row_stride + c, r < q.n ? q.k - c : 0), v[i]);
     m = __builtin_fmaxf(m, finite_max(v[i]));
   }
 #pragma unroll
@@ -126,15 +182,33 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(QuantizeWeight q) 
 
 }  // namespace
 
-hipError_t launch_quantize_rows(const QuantizeRows& q, int type, bool gated, hipStream_t stream) {
-  const int64_t nb = blocks_of(q.cols);
+namespace {
+
+template <int TYPE, bool GATED, int CU>
+hipError_t launch_rows(const QuantizeRows& q, hipStream_t stream) {
+  const int64_t nb = (blocks_of(q.cols) + CU - 1) / CU;
   const dim3 grid((unsigned)((q.rows + 15) / 16), (unsigned)(nb < 65535 ? nb : 65535));
-  auto go = [&](auto kernel) { kernel<<<grid, 256, 0, stream>>>(q); };
-  if (type == AEISU_TYPE_F16) gated ? go(quantize_rows_kernel<AEISU_TYPE_F16, true>) : go(quantize_rows_kernel<AEISU_TYPE_F16, false>);
-  else if (type == AEISU_TYPE_BF16)
-    gated ? go(quantize_rows_kernel<AEISU_TYPE_BF16, true>) : go(quantize_rows_kernel<AEISU_TYPE_BF16, false>);
-  else gated ? go(quantize_rows_kernel<AEISU_TYPE_F32, true>) : go(quantize_rows_kernel<AEISU_TYPE_F32, false>);
+  quantize_rows_kernel<TYPE, GATED, CU><<<grid, 256, 0, stream>>>(q);
   return hipGetLastError();
+}
+template <int TYPE, bool GATED>
+hipError_t launch_rows(const QuantizeRows& q, hipStream_t stream) {
+  // Two block columns a thread share the row's index and address where there are enough of them: 16,384 rows of 4096
+  // gathered 34 us against 47 with one, 35 with four; rows as they are 40.5 (5.0 TB/s) against 47 and 43.  Gated rows
+  // (14 us against 17 with two, 4096 x 2816) and rows of one block (136,640 of 128: 12.8 against 14.3 with two row
+  // groups) lose by it: they run in fewer, longer workgroups whose loads and arithmetic overlap less.
+  if constexpr (!GATED) {
+    if (blocks_of(q.cols) >= 2 && (q.rows + 15) / 16 * blocks_of(q.cols) >= 4096) return launch_rows<TYPE, GATED, 2>(q, stream);
+  }
+  return launch_rows<TYPE, GATED, 1>(q, stream);
+}
+
+}  // namespace
+
+hipError_t launch_quantize_rows(const QuantizeRows& q, int type, bool gated, hipStream_t stream) {
+  if (type == AEISU_TYPE_F16) return gated ? launch_rows<AEISU_TYPE_F16, true>(q, stream) : launch_rows<AEISU_TYPE_F16, false>(q, stream);
+  if (type == AEISU_TYPE_BF16) return gated ? launch_rows<AEISU_TYPE_BF16, true>(q, stream) : launch_rows<AEISU_TYPE_BF16, false>(q, stream);
+  return gated ? launch_rows<AEISU_TYPE_F32, true>(q, stream) : launch_rows<AEISU_TYPE_F32, false>(q, stream);
 }
 
 hipError_t launch_quantize_weight(const QuantizeWeight& q, int type, int64_t experts, hipStream_t stream) {

@@ -215,10 +215,13 @@ __device__ __forceinline__ void finish4(const aeisu_product& p, int64_t m, int64
 }
 
 // Results of a wave's MT x NT accumulators, rows m0 + 16 i + (lane & 15) below `end`, columns n0 + 16 j + 4 (lane >> 4) + r:
-// bias, activation, one rounding to the result's type.  16-bit results of two adjacent accumulators are exchanged
-// between lanes so that each lane stores eight adjacent ones.
+// bias, activation, one rounding to the result's type.
+// 16-bit results of 64 columns pass through 2 KB of LDS of the wave's own, sixteen rows at a time, so that a store
+// instruction fills eight rows' whole lines of 128 bytes; those of 32 columns are exchanged between lanes so that each
+// lane stores eight adjacent ones.
 template <int OUT, bool ACT, int MT, int NT>
-__device__ __forceinline__ void store_tile(const aeisu_product& p, int64_t m0, int64_t end, int64_t n0, const float* bias, f4 (&acc)[MT][NT]) {
+__device__ __forceinline__ void store_tile(const aeisu_product& p, int64_t m0, int64_t end, int64_t n0, const float* bias,
+                                           f4 (&acc)[MT][NT], char* stage) {
   const int lane = lane_id(), g = lane >> 4;
   constexpr int OS = OUT == AEISU_TYPE_F32 ? 4 : 2;
   if constexpr (ACT) {
@@ -241,6 +244,32 @@ __device__ __forceinline__ void store_tile(const aeisu_product& p, int64_t m0, i
         }
     }
   }
+  if constexpr (OUT != AEISU_TYPE_F32 && NT == 4) {
+    // row r of the sixteen at 128 r; its pieces of 16 bytes exchanged by r & 7 against bank conflicts
+    char* to = stage + (lane & 15) * 128 + (g & 1) * 8;
+    const char* from = stage + (lane >> 3) * 128 + ((lane ^ (lane >> 3)) & 7) * 16;
+    const int64_t n = n0 + (lane & 7) * 8, left = p.n - n;
+    int64_t m = m0 + (lane >> 3);
+    char* row = static_cast<char*>(p.out) + (m * p.out_stride + n) * OS;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        *reinterpret_cast<uint2*>(to + ((j * 2 + (g >> 1)) ^ (lane & 7)) * 16) =
+            uint2{pack16<OUT>(acc[i][j][0], acc[i][j][1]), pack16<OUT>(acc[i][j][2], acc[i][j][3])};
+#pragma unroll
+      for (int half = 0; half < 2; ++half, m += 8, row += 8 * OS * p.out_stride) {
+        const i4 v = *reinterpret_cast<const i4*>(from + half * 1024);
+        if (m < end) {
+          if (left >= 8) __builtin_memcpy(row, &v, 16);
+          else
+            for (int r = 0; r < 8; ++r)
+              if (r < left) reinterpret_cast<unsigned short*>(row)[r] = (unsigned short)(v[r >> 1] >> 16 * (r & 1));
+        }
+      }
+    }
+    return;
+  }
   int64_t m = m0 + (lane & 15);
   char* row = static_cast<char*>(p.out) + m * p.out_stride * OS;
 #pragma unroll
@@ -256,24 +285,21 @@ __device__ __forceinline__ void store_tile(const aeisu_product& p, int64_t m0, i
           for (int r = 0; r < 4; ++r)
             if (r < left) o[r] = acc[i][j][r];
       }
-    } else {
+    } else if constexpr (NT == 2) {
+      unsigned a[2], b[2];
 #pragma unroll
-      for (int j = 0; j < NT; j += 2) {
-        unsigned a[2], b[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          a[r] = pack16<OUT>(acc[i][j][2 * r], acc[i][j][2 * r + 1]);
-          b[r] = pack16<OUT>(acc[i][j + 1][2 * r], acc[i][j + 1][2 * r + 1]);
-          permlane16_swap_u(a[r], b[r]);             // lane rows 0, 2: the first accumulator's, 1, 3: the second's
-        }
-        const unsigned v[4] = {a[0], a[1], b[0], b[1]};
-        const int64_t n = n0 + (j + (g & 1)) * 16 + 8 * (g >> 1), left = m < end ? p.n - n : 0;
-        unsigned short* o = reinterpret_cast<unsigned short*>(row) + n;
-        if (left >= 8) __builtin_memcpy(o, v, 16);
-        else
-          for (int r = 0; r < 8; ++r)
-            if (r < left) o[r] = (unsigned short)(v[r >> 1] >> 16 * (r & 1));
+      for (int r = 0; r < 2; ++r) {
+        a[r] = pack16<OUT>(acc[i][0][2 * r], acc[i][0][2 * r + 1]);
+        b[r] = pack16<OUT>(acc[i][1][2 * r], acc[i][1][2 * r + 1]);
+        permlane16_swap_u(a[r], b[r]);               // lane rows 0, 2: the first accumulator's, 1, 3: the second's
       }
+      const unsigned v[4] = {a[0], a[1], b[0], b[1]};
+      const int64_t n = n0 + (g & 1) * 16 + 8 * (g >> 1), left = m < end ? p.n - n : 0;
+      unsigned short* o = reinterpret_cast<unsigned short*>(row) + n;
+      if (left >= 8) __builtin_memcpy(o, v, 16);
+      else
+        for (int r = 0; r < 8; ++r)
+          if (r < left) o[r] = (unsigned short)(v[r >> 1] >> 16 * (r & 1));
     }
   }
 }
@@ -293,7 +319,7 @@ hipError_t for_types(const aeisu_product& p, Fn fn) {
 }
 
 hipError_t launch_product_256(const aeisu_product& p, const int32_t* offsets, int experts, int cus, hipStream_t stream);
-hipError_t launch_product_128(const aeisu_product& p, const int32_t* offsets, int experts, hipStream_t stream);
+hipError_t launch_product_128(const aeisu_product& p, const int32_t* offsets, int experts, int columns, hipStream_t stream);
 hipError_t launch_product_rows(const aeisu_product& p, const int32_t* offsets, int experts, int mt, int nt, hipStream_t stream);
 
 }  // namespace aeisu
