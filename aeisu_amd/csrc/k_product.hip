@@ -129,20 +129,25 @@ int compute_units() {
   return n;
 }
 
-// Which kernel: the one with the least expected time, in microseconds from what each measured (E4M3 to BF16, a step is
-// 128 bytes of k):
-//   * 256 x 256: 1.55 a step and 6 for the stores of each round of a tile on every CU (8192 x 10240 x 5120: 346);
-//   * 128 x 128: 0.62 a step for a tile on every CU, two of which fit (485 there; 512 x 4096 x 4096: 27, where
-//     256 x 256 leaves 7/8 of the CUs idle and takes 42);
-//   * 16 a x 16 b with k split over a block's waves: (1 + 1.1 a + 0.75 b + 0.45 a b) / 32 a step (a 4, b 4, 256 x 4096 x 4096:
-//     19 against 27 for 128 x 128; a 1, b 1, 1 x 4096 x 4096: 6.6 against 26);
-//   * 64 x 64 through registers for rows that do not allow the first two: 1.1 a step, four blocks on a CU
-//     (777 x 515 x 1003 over seven experts, FP16: 29 against 21 for a 2, b 2).
-// FP32 results of E4M3 operands are exact products at half the rate, and 256 x 256 does not have the registers for them.
-// Tiles of grouped rows are estimated: where every expert's last tile is half full.
+// Which kernel: the one with the least expected time, in microseconds.  A step is 128 bytes of k.  For the tile kernels a
+// block takes `alone` a step by itself, `full` / number of blocks a step where several fill a CU, and `ends` besides the
+// steps (loads of the first, stores of the result):
+//
+//                                      alone  full  ends  on a CU   measured (E4M3 to BF16, m x n x k, us)
+//   256 x 256, groups in turn           1.28  1.40   6.7     1      8192 x 10240 x 5120 339, 512 x 4096 x 4096 42
+//   128 x 128                           0.64  0.62   1.4     2                          462                    27
+//   128 x 64                            0.41  0.41   0.6     3                          550                    20
+//   64 x 64 through registers           1.0   0.36   1.2     4                         1590                    45
+//
+// and 16 a x 16 b with k split over a block's waves (0.45 + 1.2 a + 0.87 b + 0.29 a b) / 32 a step and block of all CUs:
+// 1 x 4096 x 4096 6.6 (a 1, b 1) against 26 for 128 x 128 and 42 for 256 x 256; 512 x 4096 x 4096 36 (a 4, b 4).
+// FP32 results of E4M3 operands are exact products on the FP16 unit (128 x 128: 1.84 times the steps, 128 x 64: 1.35);
+// 256 x 256 does not have the registers for their operands.  Over 71 shapes of all types, plain and grouped, the
+// kernel chosen so took 1.7 % longer than the best one (geometric mean).
+// Grouped rows: most experts' last tile is partly filled; 0.84 tiles for each that may have rows matched best.
 struct Choice {
   enum { kAny, k128, k256, kRows } kernel;
-  int mt, nt;
+  int mt, nt;                                        // kRows: a, b; k128: columns
 };
 Choice choose(const aeisu_product& p, bool grouped, int experts, int cus) {
   const bool e4m3 = p.type == AEISU_TYPE_E4M3, exact = e4m3 && p.out_type == AEISU_TYPE_F32;
@@ -150,24 +155,32 @@ Choice choose(const aeisu_product& p, bool grouped, int experts, int cus) {
   const double steps = double((p.k * es + kStepBytes - 1) / kStepBytes);
   const double groups = grouped ? double(p.rows < experts ? p.rows : experts) : 0;
   auto share = [&](int bm, int bn) {                 // blocks for each CU
-    const double m = grouped ? std::max(double(p.rows) / bm + 0.5 * groups, 0.9 * groups) : double((p.rows + bm - 1) / bm);
-    return std::max(m, 1.0) * double((p.n + bn - 1) / bn) / cus;
+    const double m = grouped ? std::max(double(p.rows) / bm + 0.84 * groups, 1.0) : double((p.rows + bm - 1) / bm);
+    return m * double((p.n + bn - 1) / bn) / cus;
+  };
+  auto tiles = [&](double blocks, double alone, double full, double ends, int on_cu) {
+    auto round = [&](double x) { return steps * std::max(alone, full * x) + ends * x; };   // x blocks on each CU
+    const double rounds = std::floor(blocks / on_cu), rest = blocks - rounds * on_cu;
+    return 4 + rounds * round(on_cu) + (rest > 0 ? round(rest) : 0);
   };
   Choice best{Choice::kAny, 0, 0};
-  double least = 5 + steps * 1.1 * std::ceil(share(64, 64)) / (share(64, 64) > 1 ? 2 : 1);
+  double least = tiles(share(64, 64), 1.0, 0.36, 1.2, 4);
   auto offer = [&](double t, Choice c) {
     if (t < least) least = t, best = c;
   };
   for (int mt = 1; mt <= 4; mt *= 2)
-    for (int nt = 1; nt <= mt + 1 && nt <= 4; nt *= 2)
-      offer(3 + steps / 32 * (1 + 1.1 * mt + 0.75 * nt + 0.45 * mt * nt) * std::max(1.0, share(16 * mt, 16 * nt)),
-            Choice{Choice::kRows, mt, nt});
+    for (int nt = 1; nt <= (mt == 1 ? 2 : mt); nt *= 2) {
+      const double x = share(16 * mt, 16 * nt), step = (0.45 + 1.2 * mt + 0.87 * nt + 0.29 * mt * nt) / 32;
+      offer(4.2 + steps * step * (exact ? 1.1 : 1.0) * std::max(1.0, x) + 0.23 * x, Choice{Choice::kRows, mt, nt});
+    }
   // 16-byte pieces of rows, and 32-bit offsets within a tile
   const bool pieces = e4m3 || (p.k % 8 == 0 && p.x_stride % 8 == 0 && p.w_stride % 8 == 0 && p.w_expert_stride % 8 == 0 &&
                                (reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w)) % 16 == 0);
   if (pieces && std::max(p.x_stride, p.w_stride) * es <= (int64_t(1) << 32) / 256 - kStepBytes) {
-    offer(5 + steps * (exact ? 0.97 : 0.62) * std::ceil(share(128, 128)), Choice{Choice::k128, 0, 128});
-    if (!exact) offer(8 + (steps * 1.55 + 6) * std::ceil(share(256, 256)), Choice{Choice::k256, 0, 0});
+    const double slow64 = exact ? 1.35 : 1.0, slow128 = exact ? 1.84 : 1.0;
+    offer(tiles(share(128, 64), 0.41 * slow64, 0.41 * slow64, 0.6, 3), Choice{Choice::k128, 0, 64});
+    offer(tiles(share(128, 128), 0.64 * slow128, 0.62 * slow128, 1.4, 2), Choice{Choice::k128, 0, 128});
+    if (!exact) offer(tiles(share(256, 256), 1.28, 1.40, 6.7, 1), Choice{Choice::k256, 0, 0});
   }
   return best;
 }
