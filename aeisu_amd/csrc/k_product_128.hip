@@ -74,7 +74,10 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void product_tiles_k
     }
   };
 
-  f4 acc[MT][NT] = {};
+  const bool act = (p.bias && tile.expert >= 0) || p.slope != 1.f;
+  const float* bias0 = p.bias && tile.expert >= 0 ? p.bias + (int64_t)e * p.n : nullptr;
+  f4 acc[MT][NT] = {}, bias[NT];
+  if constexpr (NT == 2) load_bias<NT>(bias0, n0 + wn, p.n, bias);   // early where it costs no block on the CU
   constexpr int LOADS = CH + (kE4M3 ? WM / 64 : 0);
   constexpr int XR = MT < 4 ? MT : 4;                // fragments of x held at a time
   const int at0 = (lane & 15) * 128 + (((lane >> 4) ^ lane) & 7) * 16;
@@ -161,9 +164,9 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void product_tiles_k
       step(steps, 0.f, [] {});
     }
   }
-  const float* bias = p.bias && tile.expert >= 0 ? p.bias + (int64_t)e * p.n : nullptr;
   char* stage = lds + wave * 2048;                   // every fragment has been read, by all waves
-  if (bias || p.slope != 1.f) store_tile<OUT, true, MT, NT>(p, tile.lo + wm, tile.hi, n0 + wn, bias, acc, stage);
+  if constexpr (NT != 2) load_bias<NT>(bias0, n0 + wn, p.n, bias);
+  if (act) store_tile<OUT, true, MT, NT>(p, tile.lo + wm, tile.hi, n0 + wn, bias, acc, stage);
   else store_tile<OUT, false, MT, NT>(p, tile.lo + wm, tile.hi, n0 + wn, bias, acc, stage);
 }
 

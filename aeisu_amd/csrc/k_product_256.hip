@@ -201,8 +201,10 @@ __global__ __launch_bounds__(512, 2) void product_phased_kernel(aeisu_product p,
     at += gridDim.x / 8;
     const bool more = find(at);
     if (more) preload();
-    if (bias || p.slope != 1.f) store_tile<OUT, true, MT, NT>(p, m0, end, n0, bias, acc, stage[OUT == AEISU_TYPE_F32 ? 0 : wave]);
-    else store_tile<OUT, false, MT, NT>(p, m0, end, n0, bias, acc, stage[OUT == AEISU_TYPE_F32 ? 0 : wave]);
+    f4 b[NT];
+    load_bias<NT>(bias, n0, p.n, b);
+    if (bias || p.slope != 1.f) store_tile<OUT, true, MT, NT>(p, m0, end, n0, b, acc, stage[OUT == AEISU_TYPE_F32 ? 0 : wave]);
+    else store_tile<OUT, false, MT, NT>(p, m0, end, n0, b, acc, stage[OUT == AEISU_TYPE_F32 ? 0 : wave]);
     if (!more) return;
   }
 }

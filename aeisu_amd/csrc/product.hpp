@@ -185,6 +185,12 @@ __device__ __forceinline__ unsigned pack16(float a, float b) {
   return __builtin_bit_cast(unsigned, __builtin_convertvector((f2v){a, b}, b2v));
 }
 
+// v < 0 ? slope v : v without a branch; a slope of 0 gives 0 for minus infinity too
+__device__ __forceinline__ float activated(float v, float slope) {
+  const float least = slope > 0.f ? -__builtin_inff() : -3.402823466e38f, neg = __builtin_fmaxf(v, least) * slope;
+  return v < 0.f ? neg : v;
+}
+
 // Four results of row m from column n on: bias, activation, one rounding to the result's type.
 __device__ __forceinline__ void finish4(const aeisu_product& p, int64_t m, int64_t n, f4 v, const float* bias, bool wide) {
   const int64_t left = p.n - n;
@@ -192,8 +198,7 @@ __device__ __forceinline__ void finish4(const aeisu_product& p, int64_t m, int64
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (bias) v[i] += bias[n + (i < left ? i : 0)];
-    const float neg = p.slope > 0.f ? v[i] * p.slope : 0.f;
-    v[i] = v[i] < 0.f ? neg : v[i];
+    v[i] = activated(v[i], p.slope);
   }
   const int64_t at = m * p.out_stride + n;
   if (p.out_type == AEISU_TYPE_F32) {
@@ -214,35 +219,41 @@ __device__ __forceinline__ void finish4(const aeisu_product& p, int64_t m, int64
     for (int i = 0; i < 4 && i < left; ++i) o[i] = b[i];
 }
 
+// Bias of the columns n0 + 16 j + 4 (lane >> 4) + r, zeros without one
+template <int NT>
+__device__ __forceinline__ void load_bias(const float* bias, int64_t n0, int64_t n, f4 (&b)[NT]) {
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    b[j] = f4{0.f, 0.f, 0.f, 0.f};
+    if (bias) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int64_t at = n0 + j * 16 + 4 * (lane_id() >> 4) + r;
+        b[j][r] = bias[at < n ? at : n - 1];
+      }
+    }
+  }
+}
+
 // Results of a wave's MT x NT accumulators, rows m0 + 16 i + (lane & 15) below `end`, columns n0 + 16 j + 4 (lane >> 4) + r:
 // bias, activation, one rounding to the result's type.
 // 16-bit results of 64 columns pass through 2 KB of LDS of the wave's own, sixteen rows at a time, so that a store
 // instruction fills eight rows' whole lines of 128 bytes; those of 32 columns are exchanged between lanes so that each
 // lane stores eight adjacent ones.
 template <int OUT, bool ACT, int MT, int NT>
-__device__ __forceinline__ void store_tile(const aeisu_product& p, int64_t m0, int64_t end, int64_t n0, const float* bias,
+__device__ __forceinline__ void store_tile(const aeisu_product& p, int64_t m0, int64_t end, int64_t n0, const f4 (&bias)[NT],
                                            f4 (&acc)[MT][NT], char* stage) {
   const int lane = lane_id(), g = lane >> 4;
   constexpr int OS = OUT == AEISU_TYPE_F32 ? 4 : 2;
   if constexpr (ACT) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      f4 b = {0.f, 0.f, 0.f, 0.f};
-      if (bias) {
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int64_t n = n0 + j * 16 + 4 * g + r;
-          b[r] = bias[n < p.n ? n : p.n - 1];
+          acc[i][j][r] = activated(acc[i][j][r] + bias[j][r], p.slope);
         }
-      }
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float v = acc[i][j][r] + b[r];
-          acc[i][j][r] = v < 0.f ? (p.slope > 0.f ? v * p.slope : 0.f) : v;
-        }
-    }
   }
   if constexpr (OUT != AEISU_TYPE_F32 && NT == 4) {
     // row r of the sixteen at 128 r; its pieces of 16 bytes exchanged by r & 7 against bank conflicts
