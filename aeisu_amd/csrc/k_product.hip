@@ -14,77 +14,81 @@ namespace aeisu {
 namespace {
 
 // 64 x 64 tiles of the result, one for each block of four waves (2 x 2, each 32 x 32); operands staged through registers,
-// so rows may start at any address and end anywhere.
-template <int TYPE>
+// so rows may start at any address and end anywhere.  The pieces of the AHEAD steps after the one that is multiplied
+// are on their way into registers, and LDS holds two steps.
+template <int TYPE, bool ODD>
 __global__ __launch_bounds__(256) void product_kernel(aeisu_product p, const int32_t* offsets, int experts, int64_t ntiles) {
-  constexpr int BM = 64, BN = 64;
+  constexpr int BM = 64, BN = 64, AHEAD = 3;
   constexpr bool kE4M3 = TYPE == AEISU_TYPE_E4M3;
   constexpr int ES = kE4M3 ? 1 : 2, PER = 16 / ES, STEP = kStepBytes / ES;
-  __shared__ i4 lds[2][BM * 8];                      // x, w: 16-row pieces of 128 fragments' halves, in lane order
+  __shared__ i4 lds[2][2][BM * 8];                   // step, x or w: row r's eight pieces, exchanged by r & 7
   RowTile tile;
   if (!find_tile<BM>(offsets, experts, p.rows, (int)(blockIdx.x / ntiles), tile)) return;
   const int64_t n0 = (int64_t)(blockIdx.x % ntiles) * BN;
   const int lane = lane_id(), wave = threadIdx.x >> 6, wm = (wave & 1) * 2, wn = (wave >> 1) * 2;
   const int e = tile.expert < 0 ? 0 : tile.expert;
-  const char* xb = static_cast<const char*>(p.x);
-  const char* wb = static_cast<const char*>(p.w) + e * p.w_expert_stride * ES;
   const int64_t kb = (p.k + kBlock - 1) / kBlock;
   const float* sw = kE4M3 ? p.w_scales + (e * ((p.n + kBlock - 1) / kBlock) + n0 / kBlock) * kb : nullptr;
   f4 acc[2][2] = {};
-  const int64_t steps = tile.expert < 0 ? 0 : (p.k + STEP - 1) / STEP;
+  const int steps = tile.expert < 0 ? 0 : (int)((p.k + STEP - 1) / STEP);
   int64_t xm[2];                                     // rows whose scales this lane applies
   for (int i = 0; i < 2; ++i) {
     const int64_t m = tile.lo + (wm + i) * 16 + (lane & 15);
     xm[i] = m < tile.hi ? m : tile.hi - 1;
   }
-  for (int64_t s = 0; s < steps; ++s) {
-    i4 st[4];
+  const char* src[4];                                // this thread's two pieces of x and of w
+  int first[2];                                      // and their first column in a step
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = threadIdx.x + 256 * (i & 1);     // 512 pieces of 16 bytes an operand
-      const int row = (c >> 7) * 16 + (c & 15), piece = ((c >> 6) & 1) * 4 + ((c & 63) >> 4);
-      const int64_t left = kE4M3 ? PER : p.k - (s * STEP + piece * PER);
-      int64_t r;
-      const char* src;
-      if (i < 2) {
-        r = tile.lo + row < tile.hi ? tile.lo + row : tile.hi - 1;
-        src = xb + r * p.x_stride * ES;
-      } else {
-        r = n0 + row < p.n ? n0 + row : p.n - 1;
-        src = wb + r * p.w_stride * ES;
-      }
-      src += s * kStepBytes + piece * 16;
-      st[i] = i4{0, 0, 0, 0};
-      if (left >= PER) __builtin_memcpy(&st[i], src, 16);
-      else if (left > 0) {
-        unsigned short h[8] = {};
-        for (int j = 0; j < 8; ++j)
-          if (j < left) h[j] = reinterpret_cast<const unsigned short*>(src)[j];
-        __builtin_memcpy(&st[i], h, 16);
-      }
+  for (int i = 0; i < 4; ++i) {
+    const int c = threadIdx.x + 256 * (i & 1), row = c >> 3, piece = c & 7;   // 512 pieces of 16 bytes an operand
+    if (i < 2) {
+      const int64_t r = tile.lo + row < tile.hi ? tile.lo + row : tile.hi - 1;
+      src[i] = static_cast<const char*>(p.x) + r * p.x_stride * ES + piece * 16;
+      first[i] = piece * PER;
+    } else {
+      const int64_t r = n0 + row < p.n ? n0 + row : p.n - 1;
+      src[i] = static_cast<const char*>(p.w) + (e * p.w_expert_stride + r * p.w_stride) * ES + piece * 16;
     }
-    __syncthreads();                                 // the previous step's fragments have been read
+  }
+  auto fetch = [&](int s, Piece<ES, ODD> (&st)[4]) {
+    if (s >= steps) return;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) lds[i >> 1][threadIdx.x + 256 * (i & 1)] = st[i];
-    __syncthreads();
-    Frag x[2], w[2];
+    for (int i = 0; i < 4; ++i)
+      st[i] = load_piece<ES, ODD>(src[i] + (int64_t)s * kStepBytes, p.k - ((int64_t)s * STEP + first[i & 1]), s > 0 || first[i & 1] > 0);
+  };
+  Piece<ES, ODD> st[AHEAD][4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      x[i] = Frag{lds[0][(wm + i) * 128 + lane], lds[0][(wm + i) * 128 + 64 + lane]};
-      w[i] = Frag{lds[1][(wn + i) * 128 + lane], lds[1][(wn + i) * 128 + 64 + lane]};
-    }
+  for (int u = 0; u < AHEAD; ++u) fetch(u, st[u]);
+  for (int s0 = 0; s0 < steps; s0 += AHEAD) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float sc = 0.f;
-      if constexpr (kE4M3) sc = p.x_scales[s * p.x_scales_stride + xm[i]] * sw[s];
+    for (int u = 0; u < AHEAD; ++u) {
+      const int s = s0 + u;
+      if (s >= steps) break;
+      i4(&to)[2][BM * 8] = lds[s & 1];               // read last two steps ago, before the barrier of the step before
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if constexpr (kE4M3) {
-          const f4 part = step_e4m3_exact(w[j], x[i]);
+      for (int i = 0; i < 4; ++i) to[i >> 1][((threadIdx.x >> 3) + 32 * (i & 1)) * 8 + ((threadIdx.x ^ (threadIdx.x >> 3)) & 7)] = st[u][i].whole();
+      fetch(s + AHEAD, st[u]);
+      lds_barrier();
+      Frag x[2], w[2];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(part[r], sc, acc[i][j][r]);
-        } else {
-          acc[i][j] = step_16bit<TYPE>(w[j], x[i], acc[i][j]);
+      for (int i = 0; i < 2; ++i) {
+        const int at0 = (lane & 15) * 8 + (((lane >> 4) ^ lane) & 7), at1 = at0 ^ 4;
+        x[i] = Frag{to[0][(wm + i) * 128 + at0], to[0][(wm + i) * 128 + at1]};
+        w[i] = Frag{to[1][(wn + i) * 128 + at0], to[1][(wn + i) * 128 + at1]};
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float sc = 0.f;
+        if constexpr (kE4M3) sc = p.x_scales[s * p.x_scales_stride + xm[i]] * sw[s];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if constexpr (kE4M3) {
+            const f4 part = step_e4m3_exact(w[j], x[i]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(part[r], sc, acc[i][j][r]);
+          } else {
+            acc[i][j] = step_16bit<TYPE>(w[j], x[i], acc[i][j]);
+          }
         }
       }
     }
@@ -108,9 +112,10 @@ hipError_t launch_product_any(const aeisu_product& p, const int32_t* offsets, in
   const int64_t blocks = most_tiles(p.rows, experts, offsets != nullptr, 64) * ntiles;
   if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
   auto go = [&](auto kernel) { kernel<<<(unsigned)blocks, 256, 0, stream>>>(p, offsets, experts, ntiles); };
-  if (p.type == AEISU_TYPE_E4M3) go(product_kernel<AEISU_TYPE_E4M3>);
-  else if (p.type == AEISU_TYPE_F16) go(product_kernel<AEISU_TYPE_F16>);
-  else go(product_kernel<AEISU_TYPE_BF16>);
+  const bool odd = odd_rows(p);
+  if (p.type == AEISU_TYPE_E4M3) go(product_kernel<AEISU_TYPE_E4M3, false>);
+  else if (p.type == AEISU_TYPE_F16) odd ? go(product_kernel<AEISU_TYPE_F16, true>) : go(product_kernel<AEISU_TYPE_F16, false>);
+  else odd ? go(product_kernel<AEISU_TYPE_BF16, true>) : go(product_kernel<AEISU_TYPE_BF16, false>);
   return hipGetLastError();
 }
 
@@ -137,12 +142,13 @@ int compute_units() {
 //   256 x 256, groups in turn           1.28  1.40   6.7     1      8192 x 10240 x 5120 339, 512 x 4096 x 4096 42
 //   128 x 128                           0.64  0.62   1.4     2                          462                    27
 //   128 x 64                            0.41  0.41   0.6     3                          550                    20
-//   64 x 64 through registers           1.0   0.36   1.2     4                         1590                    45
+//   64 x 64 through registers           0.73  0.43   1.2     4      2000 x 3000 x 2001 BF16 over 8 experts 107
 //
 // and 16 a x 16 b with k split over a block's waves (0.45 + 1.2 a + 0.87 b + 0.29 a b) / 32 a step and block of all CUs:
 // 1 x 4096 x 4096 6.6 (a 1, b 1) against 26 for 128 x 128 and 42 for 256 x 256; 512 x 4096 x 4096 36 (a 4, b 4).
 // FP32 results of E4M3 operands are exact products on the FP16 unit (128 x 128: 1.84 times the steps, 128 x 64: 1.35);
-// 256 x 256 does not have the registers for their operands.  Over 71 shapes of all types, plain and grouped, the
+// 256 x 256 does not have the registers for their operands.  Few rows at odd elements: 2.2 times the steps (777 x 515 x 1003
+// FP16 over 7 experts: 18.4 with a 2, b 2, 16.5 through registers).  Over 71 shapes of all types, plain and grouped, the
 // kernel chosen so took 1.7 % longer than the best one (geometric mean).
 // Grouped rows: most experts' last tile is partly filled; 0.84 tiles for each that may have rows matched best.
 struct Choice {
@@ -164,14 +170,15 @@ Choice choose(const aeisu_product& p, bool grouped, int experts, int cus) {
     return 4 + rounds * round(on_cu) + (rest > 0 ? round(rest) : 0);
   };
   Choice best{Choice::kAny, 0, 0};
-  double least = tiles(share(64, 64), 1.0, 0.36, 1.2, 4);
+  double least = tiles(share(64, 64), 0.73, 0.43, 1.2, 4);
   auto offer = [&](double t, Choice c) {
     if (t < least) least = t, best = c;
   };
+  const double slow = exact ? 1.1 : odd_rows(p) ? 2.2 : 1.0;
   for (int mt = 1; mt <= 4; mt *= 2)
     for (int nt = 1; nt <= (mt == 1 ? 2 : mt); nt *= 2) {
       const double x = share(16 * mt, 16 * nt), step = (0.45 + 1.2 * mt + 0.87 * nt + 0.29 * mt * nt) / 32;
-      offer(4.2 + steps * step * (exact ? 1.1 : 1.0) * std::max(1.0, x) + 0.23 * x, Choice{Choice::kRows, mt, nt});
+      offer(4.2 + steps * step * slow * std::max(1.0, x) + 0.23 * x, Choice{Choice::kRows, mt, nt});
     }
   // 16-byte pieces of rows, and 32-bit offsets within a tile
   const bool pieces = e4m3 || (p.k % 8 == 0 && p.x_stride % 8 == 0 && p.w_stride % 8 == 0 && p.w_expert_stride % 8 == 0 &&

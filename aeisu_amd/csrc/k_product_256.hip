@@ -140,39 +140,49 @@ __global__ __launch_bounds__(512, 2) void product_phased_kernel(aeisu_product p,
     sc[3] = 0.f;
     barrier_with_loads();
     if (group == 1) asm volatile("s_barrier" ::: "memory");
-    for (int s = 0; s < t.steps; ++s) {
-      float sws = 0.f;
-      if constexpr (kE4M3) {
-        if ((s & 63) == 0) {
-          swv = s + lane < kb ? t.sw[s + lane] : 0.f;
-          asm volatile("" : "+v"(swv));               // waits here, not where both paths meet
+    if (wm < t.r.hi - t.r.lo) {
+      for (int s = 0; s < t.steps; ++s) {
+        float sws = 0.f;
+        if constexpr (kE4M3) {
+          if ((s & 63) == 0) {
+            swv = s + lane < kb ? t.sw[s + lane] : 0.f;
+            asm volatile("" : "+v"(swv));               // waits here, not where both paths meet
+          }
+          sws = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, swv), s & 63));
         }
-        sws = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, swv), s & 63));
+        read(s, 0);
+        if (s > 0) load_x(s + 1);
+        if constexpr (kE4M3) {
+          finish(1);
+          scales(s, 0, sws);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        multiply(0);
+        asm volatile("s_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        read(s, 1);
+        load_w(s + 2);
+        if constexpr (kE4M3) {
+          finish(0);
+          scales(s, 1, sws);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        barrier_behind<XL + WL>(s + 2, t.steps);
+        multiply(1);
+        barrier_behind<WL>(s + 2, t.steps);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      read(s, 0);
-      if (s > 0) load_x(s + 1);
-      if constexpr (kE4M3) {
-        finish(1);
-        scales(s, 0, sws);
+      if constexpr (kE4M3) finish(1);
+    } else {                                          // no rows for this group: its loads and barriers alone
+      for (int s = 0; s < t.steps; ++s) {
+        if (s > 0) load_x(s + 1);
+        asm volatile("s_barrier\n\ts_barrier" ::: "memory");
+        load_w(s + 2);
+        barrier_behind<XL + WL>(s + 2, t.steps);
+        barrier_behind<WL>(s + 2, t.steps);
       }
-      __builtin_amdgcn_sched_barrier(0);
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      multiply(0);
-      asm volatile("s_barrier" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
-      read(s, 1);
-      load_w(s + 2);
-      if constexpr (kE4M3) {
-        finish(0);
-        scales(s, 1, sws);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      barrier_behind<XL + WL>(s + 2, t.steps);
-      multiply(1);
-      barrier_behind<WL>(s + 2, t.steps);
-      __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (kE4M3) finish(1);
     if (group == 0) asm volatile("s_barrier" ::: "memory");
     if constexpr (!kE4M3) {
       const int left = (int)(p.k - (int64_t)(p.k / STEP) * STEP);

@@ -8,23 +8,7 @@ namespace {
 
 constexpr int kWaves = 8;
 
-// 16 bytes of a row of which `left` elements are its own; zeros for the others.  Rows may start anywhere.
-template <int ES>
-__device__ __forceinline__ i4 piece(const char* p, int64_t left) {
-  i4 v = {0, 0, 0, 0};
-  if (ES == 1 || left >= 8) {
-    __builtin_memcpy(&v, p, 16);
-  } else if (left > 0) {
-    unsigned short h[8] = {};
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < left) h[j] = reinterpret_cast<const unsigned short*>(p)[j];
-    __builtin_memcpy(&v, h, 16);
-  }
-  return v;
-}
-
-template <int TYPE, bool EXACT, int MT, int NT>
+template <int TYPE, bool EXACT, bool ODD, int MT, int NT>
 __global__ __launch_bounds__(64 * kWaves) void product_rows_kernel(aeisu_product p, const int32_t* offsets, int experts, int nblocks) {
   constexpr bool kE4M3 = TYPE == AEISU_TYPE_E4M3;
   constexpr int ES = kE4M3 ? 1 : 2, STEP = kStepBytes / ES, U = 2;
@@ -54,35 +38,44 @@ __global__ __launch_bounds__(64 * kWaves) void product_rows_kernel(aeisu_product
   const float* sw = kE4M3 ? p.w_scales + ((int64_t)e * ((p.n + kBlock - 1) / kBlock) + n0 / kBlock) * kb : nullptr;
   f4 acc[MT][NT] = {};
   for (int s0 = wave; s0 < steps; s0 += U * kWaves) {
-    Frag xf[U][MT], wf[U][NT];
+    Piece<ES, ODD> xf[U][MT][2], wf[U][NT][2];
     float sc[U][MT];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int s = s0 + u * kWaves < steps ? s0 + u * kWaves : steps - 1;
       const int64_t at = (int64_t)s * kStepBytes, left = p.k - (int64_t)s * STEP - g * 8;
 #pragma unroll
-      for (int j = 0; j < NT; ++j) wf[u][j] = Frag{piece<ES>(w[j] + at, left), piece<ES>(w[j] + at + 64, left - 32)};
+      for (int j = 0; j < NT; ++j) {
+        wf[u][j][0] = load_piece<ES, ODD>(w[j] + at, left, s > 0 || g > 0);
+        wf[u][j][1] = load_piece<ES, ODD>(w[j] + at + 64, left - 32, true);
+      }
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        xf[u][i] = Frag{piece<ES>(x[i] + at, left), piece<ES>(x[i] + at + 64, left - 32)};
+        xf[u][i][0] = load_piece<ES, ODD>(x[i] + at, left, s > 0 || g > 0);
+        xf[u][i][1] = load_piece<ES, ODD>(x[i] + at + 64, left - 32, true);
         if constexpr (kE4M3) sc[u][i] = sx[i][s * p.x_scales_stride] * sw[s];
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (s0 + u * kWaves >= steps) break;
+      Frag wq[NT];
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int j = 0; j < NT; ++j) wq[j] = Frag{wf[u][j][0].whole(), wf[u][j][1].whole()};
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const Frag xq{xf[u][i][0].whole(), xf[u][i][1].whole()};
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           if constexpr (kE4M3) {
-            const f4 part = EXACT ? step_e4m3_exact(wf[u][j], xf[u][i]) : step_e4m3(wf[u][j], xf[u][i]);
+            const f4 part = EXACT ? step_e4m3_exact(wq[j], xq) : step_e4m3(wq[j], xq);
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(part[r], sc[u][i], acc[i][j][r]);
           } else {
-            acc[i][j] = step_16bit<TYPE>(wf[u][j], xf[u][i], acc[i][j]);
+            acc[i][j] = step_16bit<TYPE>(wq[j], xq, acc[i][j]);
           }
         }
+      }
     }
   }
 #pragma unroll
@@ -103,21 +96,26 @@ __global__ __launch_bounds__(64 * kWaves) void product_rows_kernel(aeisu_product
   }
 }
 
-template <int TYPE, bool EXACT, int MT, int NT>
+template <int TYPE, bool EXACT, bool ODD, int MT, int NT>
 hipError_t launch(const aeisu_product& p, const int32_t* offsets, int experts, hipStream_t stream) {
   const int64_t nblocks = (p.n + 16 * NT - 1) / (16 * NT);
   const int64_t blocks = most_tiles(p.rows, experts, offsets != nullptr, 16 * MT) * nblocks;
   if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
-  product_rows_kernel<TYPE, EXACT, MT, NT><<<(unsigned)blocks, 64 * kWaves, 0, stream>>>(p, offsets, experts, (int)nblocks);
+  product_rows_kernel<TYPE, EXACT, ODD, MT, NT><<<(unsigned)blocks, 64 * kWaves, 0, stream>>>(p, offsets, experts, (int)nblocks);
   return hipGetLastError();
 }
 
 template <int MT, int NT>
 hipError_t launch_type(const aeisu_product& p, const int32_t* offsets, int experts, hipStream_t stream) {
-  if (p.type == AEISU_TYPE_F16) return launch<AEISU_TYPE_F16, false, MT, NT>(p, offsets, experts, stream);
-  if (p.type == AEISU_TYPE_BF16) return launch<AEISU_TYPE_BF16, false, MT, NT>(p, offsets, experts, stream);
-  if (p.out_type == AEISU_TYPE_F32) return launch<AEISU_TYPE_E4M3, true, MT, NT>(p, offsets, experts, stream);
-  return launch<AEISU_TYPE_E4M3, false, MT, NT>(p, offsets, experts, stream);
+  const bool odd = odd_rows(p);
+  if (p.type == AEISU_TYPE_F16)
+    return odd ? launch<AEISU_TYPE_F16, false, true, MT, NT>(p, offsets, experts, stream)
+               : launch<AEISU_TYPE_F16, false, false, MT, NT>(p, offsets, experts, stream);
+  if (p.type == AEISU_TYPE_BF16)
+    return odd ? launch<AEISU_TYPE_BF16, false, true, MT, NT>(p, offsets, experts, stream)
+               : launch<AEISU_TYPE_BF16, false, false, MT, NT>(p, offsets, experts, stream);
+  if (p.out_type == AEISU_TYPE_F32) return launch<AEISU_TYPE_E4M3, true, false, MT, NT>(p, offsets, experts, stream);
+  return launch<AEISU_TYPE_E4M3, false, false, MT, NT>(p, offsets, experts, stream);
 }
 
 }  // namespace
