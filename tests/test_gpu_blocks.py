@@ -353,6 +353,55 @@ def test_grouped_matmul_agrees_with_matmul(B):
         O.check(a, y, mag, 400, True, f"{m} rows")
 
 
+# ---- large products: a definition in 64 bits on the GPU ------------------------------------------------------------
+def on_gpu(v, cols, tiles):
+    """float64 values of codes on the GPU, from the oracle's table"""
+    from aeisu_amd import fp8
+    table = torch.from_numpy(fp8.DECODE.astype(np.float64)).cuda()
+    scale = v.scales.double()
+    wide = scale.repeat_interleave(128, -2)[..., :v.codes.shape[-2], :] if tiles else scale.t()
+    return table[v.codes[..., :cols].long()] * wide.repeat_interleave(128, -1)[..., :cols]
+
+
+@pytest.mark.parametrize("out_dtype", [F16, BF16])
+@pytest.mark.parametrize("m,n,k", [(4100, 4000, 1000), (8192, 2050, 130), (300, 20000, 2300)])
+def test_large_matmul(B, m, n, k, out_dtype):
+    g = torch.Generator("cuda").manual_seed(m)
+    x = B.quantize_rows(torch.randn(m, k, generator=g, device="cuda"))
+    w = B.quantize_weight(torch.randn(n, k, generator=g, device="cuda"))
+    bias = torch.randn(n, generator=g, device="cuda")
+    xv, wv = on_gpu(x, k, False), on_gpu(w, k, True)
+    y, mag = xv @ wv.t() + bias.double(), xv.abs() @ wv.abs().t() + bias.double().abs()
+    y = torch.where(y < 0, y * 0.1, y).cpu()
+    O.check(B.matmul(x, w, bias=bias, slope=0.1, out_dtype=out_dtype), y, mag.cpu(), k, True, f"{m}x{n}x{k}")
+
+
+@pytest.mark.parametrize("kind,k,out_dtype", [("e4m3", 900, BF16), ("e4m3", 300, F32), ("bf16", 712, BF16), ("f16", 640, F32), ("f16", 8, F16)])
+@pytest.mark.parametrize("counts", [[2000, 0, 3, 1100, 257, 1, 3000, 120], [4096, 4096], [130] * 40])
+def test_large_grouped_matmul(B, counts, kind, k, out_dtype):
+    """Enough rows for every tile height, whole and partly filled tiles, halves without rows, steps that end inside a block."""
+    e, n, t = len(counts), 1300, sum(counts)
+    g = torch.Generator("cuda").manual_seed(k)
+    x, w = torch.randn(t, k, generator=g, device="cuda"), torch.randn(e, n, k, generator=g, device="cuda")
+    if kind == "e4m3":
+        x, w = B.quantize_rows(x), B.quantize_weight(w)
+        xv, wv = on_gpu(x, k, False), on_gpu(w, k, True)
+    else:
+        x, w = (v.to(F16 if kind == "f16" else BF16) for v in (x, w))
+        xv, wv = x.double(), w.double()
+    off = offsets_of(counts)
+    out = torch.full((t + 5, n), float("nan"), dtype=out_dtype, device="cuda")
+    xs = B.QuantRows(torch.cat([x.codes, x.codes[:5]]), torch.cat([x.scales, x.scales[:, :5]], 1), k) if kind == "e4m3" \
+        else torch.cat([x, x[:5]])
+    B.grouped_matmul(xs, w, off, out=out)
+    assert not out[t:].any()
+    y = torch.zeros(t, n, dtype=torch.float64, device="cuda")
+    mag = torch.zeros_like(y)
+    for i, (lo, hi) in enumerate(zip(off.tolist(), off.tolist()[1:])):
+        y[lo:hi], mag[lo:hi] = xv[lo:hi] @ wv[i].t(), xv[lo:hi].abs() @ wv[i].abs().t()
+    O.check(out[:t], y.cpu(), mag.cpu(), k, kind == "e4m3", f"{counts[:3]} {kind} {k}")
+
+
 # ---- memory, streams, graphs ------------------------------------------------------------------------------------
 def test_offsets_past_32_bits(B):
     """Operands and results whose rows lie more than 4 GiB apart from first to last."""
