@@ -364,7 +364,7 @@ def on_gpu(v, cols, tiles):
 
 
 @pytest.mark.parametrize("out_dtype", [F16, BF16])
-@pytest.mark.parametrize("m,n,k", [(4100, 4000, 1000), (8192, 2050, 130), (300, 20000, 2300)])
+@pytest.mark.parametrize("m,n,k", [(4100, 4000, 1000), (8192, 2050, 130), (300, 20000, 2300), (20000, 16, 512), (8192, 13, 300)])
 def test_large_matmul(B, m, n, k, out_dtype):
     g = torch.Generator("cuda").manual_seed(m)
     x = B.quantize_rows(torch.randn(m, k, generator=g, device="cuda"))
@@ -376,7 +376,8 @@ def test_large_matmul(B, m, n, k, out_dtype):
     O.check(B.matmul(x, w, bias=bias, slope=0.1, out_dtype=out_dtype), y, mag.cpu(), k, True, f"{m}x{n}x{k}")
 
 
-@pytest.mark.parametrize("kind,k,out_dtype", [("e4m3", 900, BF16), ("e4m3", 300, F32), ("bf16", 712, BF16), ("f16", 640, F32), ("f16", 8, F16)])
+@pytest.mark.parametrize("kind,k,out_dtype", [("e4m3", 900, BF16), ("e4m3", 300, F32), ("bf16", 712, BF16), ("f16", 640, F32), ("f16", 8, F16), ("f16", 1003, F16),
+                                              ("bf16", 129, F32)])
 @pytest.mark.parametrize("counts", [[2000, 0, 3, 1100, 257, 1, 3000, 120], [4096, 4096], [130] * 40])
 def test_large_grouped_matmul(B, counts, kind, k, out_dtype):
     """Enough rows for every tile height, whole and partly filled tiles, halves without rows, steps that end inside a block."""
