@@ -139,17 +139,17 @@ int compute_units() {
 // steps (loads of the first, stores of the result):
 //
 //                                      alone  full  ends  on a CU   measured (E4M3 to BF16, m x n x k, us)
-//   256 x 256, groups in turn           1.28  1.40   6.7     1      8192 x 10240 x 5120 339, 512 x 4096 x 4096 42
-//   128 x 128                           0.64  0.62   1.4     2                          462                    27
+//   256 x 256, groups in turn           1.46  1.36   6.4     1      8192 x 10240 x 5120 339, 512 x 4096 x 4096 42
+//   128 x 128                           0.65  0.625  1.2     2                          462                    27
 //   128 x 64                            0.41  0.41   0.6     3                          550                    20
 //   64 x 64 through registers           0.73  0.43   1.2     4      2000 x 3000 x 2001 BF16 over 8 experts 107
 //
-// and 16 a x 16 b with k split over a block's waves (0.45 + 1.2 a + 0.87 b + 0.29 a b) / 32 a step and block of all CUs:
+// and 16 a x 16 b with k split over a block's waves (0.33 + 1.09 a + 1.19 b + 0.29 a b) / 32 a step and block of all CUs:
 // 1 x 4096 x 4096 6.6 (a 1, b 1) against 26 for 128 x 128 and 42 for 256 x 256; 512 x 4096 x 4096 36 (a 4, b 4).
-// FP32 results of E4M3 operands are exact products on the FP16 unit (128 x 128: 1.84 times the steps, 128 x 64: 1.35);
+// FP32 results of E4M3 operands are exact products on the FP16 unit (128 x 128: 1.43 times the steps, 128 x 64: 1.35);
 // 256 x 256 does not have the registers for their operands.  Few rows at odd elements: 2.2 times the steps (777 x 515 x 1003
-// FP16 over 7 experts: 18.4 with a 2, b 2, 16.5 through registers).  Over 71 shapes of all types, plain and grouped, the
-// kernel chosen so took 1.7 % longer than the best one (geometric mean).
+// FP16 over 7 experts: 18.4 with a 2, b 2, 16.5 through registers).  Over 301 shapes of all types, plain and grouped, the
+// kernel chosen so took 2.7 % longer than the best one (geometric mean).
 // Grouped rows: most experts' last tile is partly filled; 0.84 tiles for each that may have rows matched best.
 struct Choice {
   enum { kAny, k128, k256, kRows } kernel;
@@ -174,20 +174,20 @@ Choice choose(const aeisu_product& p, bool grouped, int experts, int cus) {
   auto offer = [&](double t, Choice c) {
     if (t < least) least = t, best = c;
   };
-  const double slow = exact ? 1.1 : odd_rows(p) ? 2.2 : 1.0;
+  const double slow = exact ? 1.12 : odd_rows(p) ? 2.2 : 1.0;
   for (int mt = 1; mt <= 4; mt *= 2)
     for (int nt = 1; nt <= (mt == 1 ? 2 : mt); nt *= 2) {
-      const double x = share(16 * mt, 16 * nt), step = (0.45 + 1.2 * mt + 0.87 * nt + 0.29 * mt * nt) / 32;
+      const double x = share(16 * mt, 16 * nt), step = (0.33 + 1.09 * mt + 1.19 * nt + 0.29 * mt * nt) / 32;
       offer(4.2 + steps * step * slow * std::max(1.0, x) + 0.23 * x, Choice{Choice::kRows, mt, nt});
     }
   // 16-byte pieces of rows, and 32-bit offsets within a tile
   const bool pieces = e4m3 || (p.k % 8 == 0 && p.x_stride % 8 == 0 && p.w_stride % 8 == 0 && p.w_expert_stride % 8 == 0 &&
                                (reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w)) % 16 == 0);
   if (pieces && std::max(p.x_stride, p.w_stride) * es <= (int64_t(1) << 32) / 256 - kStepBytes) {
-    const double slow64 = exact ? 1.35 : 1.0, slow128 = exact ? 1.84 : 1.0;
+    const double slow64 = exact ? 1.35 : 1.0, slow128 = exact ? 1.43 : 1.0;
     offer(tiles(share(128, 64), 0.41 * slow64, 0.41 * slow64, 0.6, 3), Choice{Choice::k128, 0, 64});
-    offer(tiles(share(128, 128), 0.64 * slow128, 0.62 * slow128, 1.4, 2), Choice{Choice::k128, 0, 128});
-    if (!exact) offer(tiles(share(256, 256), 1.28, 1.40, 6.7, 1), Choice{Choice::k256, 0, 0});
+    offer(tiles(share(128, 128), 0.65 * slow128, 0.625 * slow128, 1.2, 2), Choice{Choice::k128, 0, 128});
+    if (!exact) offer(tiles(share(256, 256), 1.46, 1.36, 6.4, 1), Choice{Choice::k256, 0, 0});
   }
   return best;
 }
