@@ -16,10 +16,10 @@ namespace {
 // 64 x 64 tiles of the result, one for each block of four waves (2 x 2, each 32 x 32); operands staged through registers,
 // so rows may start at any address and end anywhere.  The pieces of the AHEAD steps after the one that is multiplied
 // are on their way into registers, and LDS holds two steps.
-template <int TYPE, bool ODD>
+template <int TYPE>
 __global__ __launch_bounds__(256) void product_kernel(aeisu_product p, const int32_t* offsets, int experts, int64_t ntiles) {
   constexpr int BM = 64, BN = 64, AHEAD = 3;
-  constexpr bool kE4M3 = TYPE == AEISU_TYPE_E4M3;
+  constexpr bool kE4M3 = TYPE == AEISU_TYPE_E4M3, ODD = !kE4M3;
   constexpr int ES = kE4M3 ? 1 : 2, PER = 16 / ES, STEP = kStepBytes / ES;
   __shared__ i4 lds[2][2][BM * 8];                   // step, x or w: row r's eight pieces, exchanged by r & 7
   RowTile tile;
@@ -112,10 +112,9 @@ hipError_t launch_product_any(const aeisu_product& p, const int32_t* offsets, in
   const int64_t blocks = most_tiles(p.rows, experts, offsets != nullptr, 64) * ntiles;
   if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
   auto go = [&](auto kernel) { kernel<<<(unsigned)blocks, 256, 0, stream>>>(p, offsets, experts, ntiles); };
-  const bool odd = odd_rows(p);
-  if (p.type == AEISU_TYPE_E4M3) go(product_kernel<AEISU_TYPE_E4M3, false>);
-  else if (p.type == AEISU_TYPE_F16) odd ? go(product_kernel<AEISU_TYPE_F16, true>) : go(product_kernel<AEISU_TYPE_F16, false>);
-  else odd ? go(product_kernel<AEISU_TYPE_BF16, true>) : go(product_kernel<AEISU_TYPE_BF16, false>);
+  if (p.type == AEISU_TYPE_E4M3) go(product_kernel<AEISU_TYPE_E4M3>);
+  else if (p.type == AEISU_TYPE_F16) go(product_kernel<AEISU_TYPE_F16>);
+  else go(product_kernel<AEISU_TYPE_BF16>);
   return hipGetLastError();
 }
 
@@ -135,25 +134,28 @@ int compute_units() {
 }
 
 // Which kernel: the one with the least expected time, in microseconds.  A step is 128 bytes of k.  For the tile kernels a
-// block takes `alone` a step by itself, `full` / number of blocks a step where several fill a CU, and `ends` besides the
+// block takes `alone` a step by itself, `full` times the blocks on its CU where several fill it, and `ends` besides the
 // steps (loads of the first, stores of the result):
 //
 //                                      alone  full  ends  on a CU   measured (E4M3 to BF16, m x n x k, us)
-//   256 x 256, groups in turn           1.46  1.36   6.4     1      8192 x 10240 x 5120 339, 512 x 4096 x 4096 42
-//   128 x 128                           0.65  0.625  1.2     2                          462                    27
-//   128 x 64                            0.41  0.41   0.6     3                          550                    20
+//   256 x 256, groups in turn           1.38  1.38   5.7     1      8192 x 10240 x 5120 339, 512 x 4096 x 4096 42
+//   128 x 128                           0.60  0.585  1.0     2                          462                    27
+//   128 x 64                            0.37  0.39   0.53    3                          550                    20
 //   64 x 64 through registers           0.73  0.43   1.2     4      2000 x 3000 x 2001 BF16 over 8 experts 107
 //
-// and 16 a x 16 b with k split over a block's waves (0.33 + 1.09 a + 1.19 b + 0.29 a b) / 32 a step and block of all CUs:
-// 1 x 4096 x 4096 6.6 (a 1, b 1) against 26 for 128 x 128 and 42 for 256 x 256; 512 x 4096 x 4096 36 (a 4, b 4).
-// FP32 results of E4M3 operands are exact products on the FP16 unit (128 x 128: 1.43 times the steps, 128 x 64: 1.35);
-// 256 x 256 does not have the registers for their operands.  Few rows at odd elements: 2.2 times the steps (777 x 515 x 1003
-// FP16 over 7 experts: 18.4 with a 2, b 2, 16.5 through registers).  Over 301 shapes of all types, plain and grouped, the
-// kernel chosen so took 2.7 % longer than the best one (geometric mean).
-// Grouped rows: most experts' last tile is partly filled; 0.84 tiles for each that may have rows matched best.
+// and 16 a x 16 b with k split over a block's waves (0.34 + 0.60 a + 0.70 b + 0.13 a b) / 32 a step and block of all CUs:
+// 1 x 4096 x 4096 6.4 (a 1, b 1) against 26 for 128 x 128 and 42 for 256 x 256; 100 x 4096 x 4096 8.6 (a 4, b 2) against 26 for
+// 128 x 128; 512 x 4096 x 4096 26 (a 4, b 4) against 20 for 128 x 64.
+// FP32 results of E4M3 operands are exact products on the FP16 unit (128 x 128: 1.79 times the steps, 128 x 64: 1.32);
+// 256 x 256 does not have the registers for their operands.  Few rows at odd elements: 3.6 times the steps (777 x 515 x 1003
+// FP16 over 7 experts: 18.4 with a 2, b 2, 16.5 through registers), and no registers for a 4, b 4.
+// Grouped rows: most experts' last tile is partly filled; 0.97 tiles for each that may have rows matched best.
+// Over 301 shapes of all types, plain and grouped, the kernel chosen so took 2.9 % longer than the best one (geometric
+// mean).
 struct Choice {
   enum { kAny, k128, k256, kRows } kernel;
   int mt, nt;                                        // kRows: a, b; k128: columns
+  bool odd;                                          // kRows: from memory into registers
 };
 Choice choose(const aeisu_product& p, bool grouped, int experts, int cus) {
   const bool e4m3 = p.type == AEISU_TYPE_E4M3, exact = e4m3 && p.out_type == AEISU_TYPE_F32;
@@ -161,33 +163,37 @@ Choice choose(const aeisu_product& p, bool grouped, int experts, int cus) {
   const double steps = double((p.k * es + kStepBytes - 1) / kStepBytes);
   const double groups = grouped ? double(p.rows < experts ? p.rows : experts) : 0;
   auto share = [&](int bm, int bn) {                 // blocks for each CU
-    const double m = grouped ? std::max(double(p.rows) / bm + 0.84 * groups, 1.0) : double((p.rows + bm - 1) / bm);
+    const double m = grouped ? std::max(double(p.rows) / bm + 0.97 * groups, 1.0) : double((p.rows + bm - 1) / bm);
     return m * double((p.n + bn - 1) / bn) / cus;
   };
   auto tiles = [&](double blocks, double alone, double full, double ends, int on_cu) {
     auto round = [&](double x) { return steps * std::max(alone, full * x) + ends * x; };   // x blocks on each CU
     const double rounds = std::floor(blocks / on_cu), rest = blocks - rounds * on_cu;
-    return 4 + rounds * round(on_cu) + (rest > 0 ? round(rest) : 0);
+    return 4.5 + rounds * round(on_cu) + (rest > 0 ? round(rest) : 0);
   };
-  Choice best{Choice::kAny, 0, 0};
+  Choice best{Choice::kAny, 0, 0, false};
   double least = tiles(share(64, 64), 0.73, 0.43, 1.2, 4);
   auto offer = [&](double t, Choice c) {
     if (t < least) least = t, best = c;
   };
-  const double slow = exact ? 1.12 : odd_rows(p) ? 2.2 : 1.0;
-  for (int mt = 1; mt <= 4; mt *= 2)
-    for (int nt = 1; nt <= (mt == 1 ? 2 : mt); nt *= 2) {
-      const double x = share(16 * mt, 16 * nt), step = (0.33 + 1.09 * mt + 1.19 * nt + 0.29 * mt * nt) / 32;
-      offer(4.2 + steps * step * slow * std::max(1.0, x) + 0.23 * x, Choice{Choice::kRows, mt, nt});
-    }
   // 16-byte pieces of rows, and 32-bit offsets within a tile
   const bool pieces = e4m3 || (p.k % 8 == 0 && p.x_stride % 8 == 0 && p.w_stride % 8 == 0 && p.w_expert_stride % 8 == 0 &&
                                (reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w)) % 16 == 0);
-  if (pieces && std::max(p.x_stride, p.w_stride) * es <= (int64_t(1) << 32) / 256 - kStepBytes) {
-    const double slow64 = exact ? 1.35 : 1.0, slow128 = exact ? 1.43 : 1.0;
-    offer(tiles(share(128, 64), 0.41 * slow64, 0.41 * slow64, 0.6, 3), Choice{Choice::k128, 0, 64});
-    offer(tiles(share(128, 128), 0.65 * slow128, 0.625 * slow128, 1.2, 2), Choice{Choice::k128, 0, 128});
-    if (!exact) offer(tiles(share(256, 256), 1.46, 1.36, 6.4, 1), Choice{Choice::k256, 0, 0});
+  const int64_t apart = std::max(p.x_stride, p.w_stride) * es;
+  auto near = [&](int rows) { return pieces && apart <= (int64_t(1) << 32) / rows - kStepBytes; };
+  const double slow = exact ? 1.14 : e4m3 ? 1.0 : pieces ? 1.07 : 3.6;
+  for (int mt = 1; mt <= 4; mt *= 2)
+    for (int nt = 1; nt <= (mt == 1 ? 2 : mt); nt *= 2) {
+      const bool odd = !near(16 * std::max(mt, nt));
+      if (odd && (e4m3 || mt * nt == 16)) continue;
+      const double x = share(16 * mt, 16 * nt), step = (0.34 + 0.60 * mt + 0.70 * nt + 0.13 * mt * nt) / 32;
+      offer(4.2 + steps * step * slow * std::max(1.0, x) + (0.2 + 0.117 * mt * nt) * x, Choice{Choice::kRows, mt, nt, odd});
+    }
+  if (near(256)) {
+    const double slow64 = exact ? 1.32 : 1.0, slow128 = exact ? 1.79 : 1.0;
+    offer(tiles(share(128, 64), 0.37 * slow64, 0.39 * slow64, 0.53, 3), Choice{Choice::k128, 0, 64, false});
+    offer(tiles(share(128, 128), 0.60 * slow128, 0.585 * slow128, 1.0, 2), Choice{Choice::k128, 0, 128, false});
+    if (!exact) offer(tiles(share(256, 256), 1.38, 1.38, 5.7, 1), Choice{Choice::k256, 0, 0, false});
   }
   return best;
 }
@@ -200,7 +206,7 @@ hipError_t launch_product(const aeisu_product& p, const int32_t* offsets, int ex
   switch (c.kernel) {
     case Choice::k256: return launch_product_256(p, offsets, experts, cus, stream);
     case Choice::k128: return launch_product_128(p, offsets, experts, c.nt, stream);
-    case Choice::kRows: return launch_product_rows(p, offsets, experts, c.mt, c.nt, stream);
+    case Choice::kRows: return launch_product_rows(p, offsets, experts, c.mt, c.nt, c.odd, stream);
     default: return launch_product_any(p, offsets, experts, stream);
   }
 }

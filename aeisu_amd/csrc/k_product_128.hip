@@ -1,6 +1,4 @@
 // Products in tiles of 128 x 128 (four waves of 64 x 64, two blocks on a CU) or 128 x 64 (64 x 32, three blocks).
-#include <atomic>
-
 #include "product.hpp"
 
 namespace aeisu {
@@ -180,17 +178,8 @@ hipError_t launch(const aeisu_product& p, const int32_t* offsets, int experts, h
   constexpr int WAVES = (BM / WM) * (BN / WN), STAGE = (BM + BN) * kStepBytes + (TYPE == AEISU_TYPE_E4M3 ? WAVES * WM * 4 : 0);
   constexpr int STEP = TYPE == AEISU_TYPE_E4M3 ? kStepBytes : kStepBytes / 2;
   if constexpr (2 * STAGE > 65536) {
-    static std::atomic<uint64_t> allowed;              // devices on which this kernel may have so much LDS
-    int device = 0;
-    hipError_t e = hipGetDevice(&device);
+    const hipError_t e = allow_lds<product_tiles_kernel<TYPE, OUT, BM, BN, WM, WN>>(2 * STAGE);
     if (e != hipSuccess) return e;
-    const uint64_t bit = uint64_t(1) << (device & 63);
-    if (device > 63 || !(allowed.load(std::memory_order_relaxed) & bit)) {
-      e = hipFuncSetAttribute(reinterpret_cast<const void*>(&product_tiles_kernel<TYPE, OUT, BM, BN, WM, WN>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, 2 * STAGE);
-      if (e != hipSuccess) return e;
-      allowed.fetch_or(bit, std::memory_order_relaxed);
-    }
   }
   product_tiles_kernel<TYPE, OUT, BM, BN, WM, WN>
       <<<(unsigned)blocks, 64 * WAVES, p.k > STEP ? 2 * STAGE : STAGE, stream>>>(p, offsets, experts, (int)ntiles);

@@ -1,6 +1,7 @@
-// Products of few rows: blocks of 16 MT rows x 16 NT columns, the columns of the operands split over a block's eight
-// waves.  Each wave reads its fragments from memory into registers and keeps sums of its own, which meet in LDS in the
-// order of the waves.
+// Products of few rows: blocks of 16 MT rows x 16 NT columns of the result, k split over a block's eight waves, so that few
+// blocks keep the whole memory system busy.  Each wave keeps sums of its own, which meet in LDS in the order of the waves.
+// Bound by the weights' bytes where rows are few (1 x 10240 x 8000 E4M3: 16.5 us, 5.0 TB/s; 256 rows over 64 experts of
+// 2048 x 2048: 45 us, 5.9 TB/s), by L2 and the loads' issue beyond.
 #include "product.hpp"
 
 namespace aeisu {
@@ -8,52 +9,161 @@ namespace {
 
 constexpr int kWaves = 8;
 
-template <int TYPE, bool EXACT, bool ODD, int MT, int NT>
-__global__ __launch_bounds__(64 * kWaves) void product_rows_kernel(aeisu_product p, const int32_t* offsets, int experts, int nblocks) {
+// The waves' sums, joined and finished.  The first `used` waves have any; LDS is free for them.
+template <int MT, int NT>
+__device__ __forceinline__ void join(const aeisu_product& p, const RowTile& tile, int64_t n0, int wave, int used, const float* bias,
+                                     const f4 (&acc)[MT][NT], f4* sums) {
+  const int lane = lane_id();
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) sums[(wave * MT * NT + i * NT + j) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  const size_t vec = p.out_type == AEISU_TYPE_F32 ? 16 : 8;
+  const bool wide = (reinterpret_cast<uintptr_t>(p.out) % vec) == 0 && p.out_stride % 4 == 0;
+  for (int t = wave; t < MT * NT; t += kWaves) {
+    const int64_t m = tile.lo + (t / NT) * 16 + (lane & 15);
+    if (m >= tile.hi) continue;
+    f4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int q = 0; q < used; ++q) v += sums[(q * MT * NT + t) * 64 + lane];
+    finish4(p, m, n0 + (t % NT) * 16 + 4 * (lane >> 4), v, bias, wide);
+  }
+}
+
+// A wave's operands of a step pass through LDS of its own, eight rows' whole lines an instruction: fragments read from
+// memory take sixteen rows' half lines, and the units that issue loads bind then (100 x 4096 x 4096 E4M3: 15.3 us so,
+// 8.6 through LDS; 64 x 2048 x 2048 BF16 8.4 and 5.8).  A wave waits for nothing but its own loads, and the next
+// step's are under way while it multiplies.
+template <int TYPE, bool EXACT, int MT, int NT>
+__global__ __launch_bounds__(64 * kWaves, 2) void product_rows_kernel(aeisu_product p, const int32_t* offsets, int experts, int nblocks) {
   constexpr bool kE4M3 = TYPE == AEISU_TYPE_E4M3;
-  constexpr int ES = kE4M3 ? 1 : 2, STEP = kStepBytes / ES, U = 2;
-  __shared__ f4 sums[kWaves][MT * NT][64];
+  constexpr int ES = kE4M3 ? 1 : 2, STEP = kStepBytes / ES, CH = 2 * (MT + NT), OWN = CH * 1024;
+  extern __shared__ __align__(1024) char lds[];
   RowTile tile;
   if (!find_tile<16 * MT>(offsets, experts, p.rows, (int)(blockIdx.x / nblocks), tile)) return;
   const int64_t n0 = (int64_t)(blockIdx.x % nblocks) * 16 * NT;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
   const int e = tile.expert < 0 ? 0 : tile.expert;
   const int kb = (int)((p.k + kBlock - 1) / kBlock);
-  const int steps = tile.expert < 0 ? 0 : (int)((p.k + STEP - 1) / STEP);
-  const char *x[MT], *w[NT];
+  const int steps = __builtin_amdgcn_readfirstlane(tile.expert < 0 ? 0 : (int)((p.k + STEP - 1) / STEP));
+  const char* xb = uniform(static_cast<const char*>(p.x) + tile.lo * p.x_stride * ES);
+  const char* wb = uniform(static_cast<const char*>(p.w) + (e * p.w_expert_stride + n0 * p.w_stride) * ES);
+  const int xlast = (int)(tile.hi - tile.lo) - 1, wlast = (int)(p.n - n0 < 16 * NT ? p.n - n0 : 16 * NT) - 1;
+  const int piece = (lane ^ (lane >> 3)) & 7;         // of its row's eight, exchanged by row against bank conflicts
+  unsigned off[CH];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int row = (i < 2 * MT ? i : i - 2 * MT) * 8 + (lane >> 3), last = i < 2 * MT ? xlast : wlast;
+    off[i] = (unsigned)((row < last ? row : last) * (i < 2 * MT ? p.x_stride : p.w_stride) * ES) + piece * 16;
+  }
   const float* sx[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
-    int64_t m = tile.lo + i * 16 + (lane & 15);
-    m = m < tile.hi ? m : tile.hi - 1;
-    x[i] = static_cast<const char*>(p.x) + m * p.x_stride * ES + g * 16;
-    sx[i] = kE4M3 ? p.x_scales + m : nullptr;
+    const int64_t m = tile.lo + i * 16 + (lane & 15);
+    sx[i] = kE4M3 ? p.x_scales + (m < tile.hi ? m : tile.hi - 1) : nullptr;
+  }
+  const float* sw = kE4M3 ? p.w_scales + ((int64_t)e * ((p.n + kBlock - 1) / kBlock) + n0 / kBlock) * kb : nullptr;
+  char* own = lds + wave * OWN;
+  const unsigned own0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds + wave * OWN;
+  auto load = [&](int s) {
+    const int64_t left = p.k - (int64_t)s * STEP;
+    if (!kE4M3 && left < STEP) {                       // the row ends inside: pieces past its end are zero
+      if (left <= 0) return;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const char* a = (i < 2 * MT ? xb : wb) + (int64_t)s * kStepBytes + off[i];
+        dma16_from(own0 + i * 1024, piece * 8 < left ? a : reinterpret_cast<const char*>(zero_piece));
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < CH; ++i) dma16(own0 + i * 1024, (i < 2 * MT ? xb : wb) + (int64_t)s * kStepBytes, off[i], s, steps);
+  };
+  const int at0 = (lane & 15) * kStepBytes + ((g ^ lane) & 7) * 16, at1 = at0 ^ 64;
+  auto frag = [&](int tile16) {
+    return Frag{*reinterpret_cast<const i4*>(own + at0 + tile16 * 2048), *reinterpret_cast<const i4*>(own + at1 + tile16 * 2048)};
+  };
+  f4 acc[MT][NT] = {};
+  float xs[MT], ws = 0.f;                              // the next step's scales
+  auto scales = [&](int s) {
+    if constexpr (kE4M3) {
+      s = s < steps ? s : steps - 1;
+      ws = sw[s];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) xs[i] = sx[i][s * p.x_scales_stride];
+    }
+  };
+  load(wave);
+  if (wave < steps) scales(wave);
+  for (int s = wave; s < steps; s += kWaves) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    Frag x[MT], w[NT];
+    float sc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) x[i] = frag(i);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) w[j] = frag(MT + j);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sc[i] = kE4M3 ? xs[i] * ws : 0.f;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the fragments are read: their place may be filled again
+    load(s + kWaves);
+    scales(s + kWaves);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        if constexpr (kE4M3) {
+          const f4 part = EXACT ? step_e4m3_exact(w[j], x[i]) : step_e4m3(w[j], x[i]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(part[r], sc[i], acc[i][j][r]);
+        } else {
+          acc[i][j] = step_16bit<TYPE>(w[j], x[i], acc[i][j]);
+        }
+      }
+  }
+  __syncthreads();                                     // every wave's fragments are read: the sums take their place
+  join<MT, NT>(p, tile, n0, wave, steps < kWaves ? steps : kWaves, p.bias && tile.expert >= 0 ? p.bias + (int64_t)e * p.n : nullptr, acc,
+               reinterpret_cast<f4*>(lds));
+}
+
+// 16-bit rows that do not all start at a multiple of 16 bytes: fragments from memory into registers, two steps at a time.
+template <int TYPE, int MT, int NT>
+__global__ __launch_bounds__(64 * kWaves) void product_odd_rows_kernel(aeisu_product p, const int32_t* offsets, int experts, int nblocks) {
+  constexpr int STEP = kStepBytes / 2, U = 2;
+  __shared__ f4 sums[kWaves * MT * NT * 64];
+  RowTile tile;
+  if (!find_tile<16 * MT>(offsets, experts, p.rows, (int)(blockIdx.x / nblocks), tile)) return;
+  const int64_t n0 = (int64_t)(blockIdx.x % nblocks) * 16 * NT;
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
+  const int e = tile.expert < 0 ? 0 : tile.expert;
+  const int steps = tile.expert < 0 ? 0 : (int)((p.k + STEP - 1) / STEP);
+  const char *x[MT], *w[NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int64_t m = tile.lo + i * 16 + (lane & 15);
+    x[i] = static_cast<const char*>(p.x) + (m < tile.hi ? m : tile.hi - 1) * p.x_stride * 2 + g * 16;
   }
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
-    int64_t n = n0 + j * 16 + (lane & 15);
-    n = n < p.n ? n : p.n - 1;
-    w[j] = static_cast<const char*>(p.w) + (e * p.w_expert_stride + n * p.w_stride) * ES + g * 16;
+    const int64_t n = n0 + j * 16 + (lane & 15);
+    w[j] = static_cast<const char*>(p.w) + (e * p.w_expert_stride + (n < p.n ? n : p.n - 1) * p.w_stride) * 2 + g * 16;
   }
-  const float* sw = kE4M3 ? p.w_scales + ((int64_t)e * ((p.n + kBlock - 1) / kBlock) + n0 / kBlock) * kb : nullptr;
   f4 acc[MT][NT] = {};
   for (int s0 = wave; s0 < steps; s0 += U * kWaves) {
-    Piece<ES, ODD> xf[U][MT][2], wf[U][NT][2];
-    float sc[U][MT];
+    Piece<2, true> xf[U][MT][2], wf[U][NT][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int s = s0 + u * kWaves < steps ? s0 + u * kWaves : steps - 1;
       const int64_t at = (int64_t)s * kStepBytes, left = p.k - (int64_t)s * STEP - g * 8;
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        wf[u][j][0] = load_piece<ES, ODD>(w[j] + at, left, s > 0 || g > 0);
-        wf[u][j][1] = load_piece<ES, ODD>(w[j] + at + 64, left - 32, true);
+        wf[u][j][0] = load_piece<2, true>(w[j] + at, left, s > 0 || g > 0);
+        wf[u][j][1] = load_piece<2, true>(w[j] + at + 64, left - 32, true);
       }
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        xf[u][i][0] = load_piece<ES, ODD>(x[i] + at, left, s > 0 || g > 0);
-        xf[u][i][1] = load_piece<ES, ODD>(x[i] + at + 64, left - 32, true);
-        if constexpr (kE4M3) sc[u][i] = sx[i][s * p.x_scales_stride] * sw[s];
+        xf[u][i][0] = load_piece<2, true>(x[i] + at, left, s > 0 || g > 0);
+        xf[u][i][1] = load_piece<2, true>(x[i] + at + 64, left - 32, true);
       }
     }
 #pragma unroll
@@ -66,65 +176,49 @@ __global__ __launch_bounds__(64 * kWaves) void product_rows_kernel(aeisu_product
       for (int i = 0; i < MT; ++i) {
         const Frag xq{xf[u][i][0].whole(), xf[u][i][1].whole()};
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          if constexpr (kE4M3) {
-            const f4 part = EXACT ? step_e4m3_exact(wq[j], xq) : step_e4m3(wq[j], xq);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(part[r], sc[u][i], acc[i][j][r]);
-          } else {
-            acc[i][j] = step_16bit<TYPE>(wq[j], xq, acc[i][j]);
-          }
-        }
+        for (int j = 0; j < NT; ++j) acc[i][j] = step_16bit<TYPE>(wq[j], xq, acc[i][j]);
       }
     }
   }
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) sums[wave][i * NT + j][lane] = acc[i][j];
-  __syncthreads();
-  const size_t vec = p.out_type == AEISU_TYPE_F32 ? 16 : 8;
-  const bool wide = (reinterpret_cast<uintptr_t>(p.out) % vec) == 0 && p.out_stride % 4 == 0;
-  const float* bias = p.bias && tile.expert >= 0 ? p.bias + (int64_t)e * p.n : nullptr;
-  const int used = steps < kWaves ? steps : kWaves;
-  for (int t = wave; t < MT * NT; t += kWaves) {
-    const int64_t m = tile.lo + (t / NT) * 16 + (lane & 15);
-    if (m >= tile.hi) continue;
-    f4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int q = 0; q < used; ++q) v += sums[q][t][lane];
-    finish4(p, m, n0 + (t % NT) * 16 + 4 * g, v, bias, wide);
-  }
+  join<MT, NT>(p, tile, n0, wave, steps < kWaves ? steps : kWaves, p.bias && tile.expert >= 0 ? p.bias + (int64_t)e * p.n : nullptr, acc, sums);
 }
 
-template <int TYPE, bool EXACT, bool ODD, int MT, int NT>
-hipError_t launch(const aeisu_product& p, const int32_t* offsets, int experts, hipStream_t stream) {
+template <int TYPE, bool EXACT, int MT, int NT>
+hipError_t launch(const aeisu_product& p, const int32_t* offsets, int experts, bool odd, hipStream_t stream) {
   const int64_t nblocks = (p.n + 16 * NT - 1) / (16 * NT);
   const int64_t blocks = most_tiles(p.rows, experts, offsets != nullptr, 16 * MT) * nblocks;
   if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
-  product_rows_kernel<TYPE, EXACT, ODD, MT, NT><<<(unsigned)blocks, 64 * kWaves, 0, stream>>>(p, offsets, experts, (int)nblocks);
+  if constexpr (TYPE != AEISU_TYPE_E4M3) {
+    if (odd) {
+      if constexpr (MT * NT == 16) return hipErrorInvalidValue;   // not chosen: its operands do not fit the registers
+      else product_odd_rows_kernel<TYPE, MT, NT><<<(unsigned)blocks, 64 * kWaves, 0, stream>>>(p, offsets, experts, (int)nblocks);
+      return hipGetLastError();
+    }
+  }
+  constexpr int OWN = 2 * (MT + NT) * 1024, SUMS = MT * NT * 1024, LDS = kWaves * (OWN > SUMS ? OWN : SUMS);
+  if constexpr (LDS > 65536) {
+    const hipError_t r = allow_lds<product_rows_kernel<TYPE, EXACT, MT, NT>>(LDS);
+    if (r != hipSuccess) return r;
+  }
+  product_rows_kernel<TYPE, EXACT, MT, NT><<<(unsigned)blocks, 64 * kWaves, LDS, stream>>>(p, offsets, experts, (int)nblocks);
   return hipGetLastError();
 }
 
 template <int MT, int NT>
-hipError_t launch_type(const aeisu_product& p, const int32_t* offsets, int experts, hipStream_t stream) {
-  const bool odd = odd_rows(p);
-  if (p.type == AEISU_TYPE_F16)
-    return odd ? launch<AEISU_TYPE_F16, false, true, MT, NT>(p, offsets, experts, stream)
-               : launch<AEISU_TYPE_F16, false, false, MT, NT>(p, offsets, experts, stream);
-  if (p.type == AEISU_TYPE_BF16)
-    return odd ? launch<AEISU_TYPE_BF16, false, true, MT, NT>(p, offsets, experts, stream)
-               : launch<AEISU_TYPE_BF16, false, false, MT, NT>(p, offsets, experts, stream);
-  if (p.out_type == AEISU_TYPE_F32) return launch<AEISU_TYPE_E4M3, true, false, MT, NT>(p, offsets, experts, stream);
-  return launch<AEISU_TYPE_E4M3, false, false, MT, NT>(p, offsets, experts, stream);
+hipError_t launch_type(const aeisu_product& p, const int32_t* offsets, int experts, bool odd, hipStream_t stream) {
+  if (p.type == AEISU_TYPE_F16) return launch<AEISU_TYPE_F16, false, MT, NT>(p, offsets, experts, odd, stream);
+  if (p.type == AEISU_TYPE_BF16) return launch<AEISU_TYPE_BF16, false, MT, NT>(p, offsets, experts, odd, stream);
+  if (p.out_type == AEISU_TYPE_F32) return launch<AEISU_TYPE_E4M3, true, MT, NT>(p, offsets, experts, odd, stream);
+  return launch<AEISU_TYPE_E4M3, false, MT, NT>(p, offsets, experts, odd, stream);
 }
 
 }  // namespace
 
-hipError_t launch_product_rows(const aeisu_product& p, const int32_t* offsets, int experts, int mt, int nt, hipStream_t stream) {
-  if (mt == 1) return nt == 1 ? launch_type<1, 1>(p, offsets, experts, stream) : launch_type<1, 2>(p, offsets, experts, stream);
-  if (mt == 2) return nt == 1 ? launch_type<2, 1>(p, offsets, experts, stream) : launch_type<2, 2>(p, offsets, experts, stream);
-  if (nt == 1) return launch_type<4, 1>(p, offsets, experts, stream);
-  return nt == 2 ? launch_type<4, 2>(p, offsets, experts, stream) : launch_type<4, 4>(p, offsets, experts, stream);
+hipError_t launch_product_rows(const aeisu_product& p, const int32_t* offsets, int experts, int mt, int nt, bool odd, hipStream_t stream) {
+  if (mt == 1) return nt == 1 ? launch_type<1, 1>(p, offsets, experts, odd, stream) : launch_type<1, 2>(p, offsets, experts, odd, stream);
+  if (mt == 2) return nt == 1 ? launch_type<2, 1>(p, offsets, experts, odd, stream) : launch_type<2, 2>(p, offsets, experts, odd, stream);
+  if (nt == 1) return launch_type<4, 1>(p, offsets, experts, odd, stream);
+  return nt == 2 ? launch_type<4, 2>(p, offsets, experts, odd, stream) : launch_type<4, 4>(p, offsets, experts, odd, stream);
 }
 
 }  // namespace aeisu

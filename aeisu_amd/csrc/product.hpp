@@ -3,6 +3,8 @@
 // All products run with the weights as the matrix unit's first operand, so an accumulator lane holds one row of x and
 // four consecutive columns of the result: its scale is one number and its four results leave in one store.
 #pragma once
+#include <atomic>
+
 #include "blocks.hpp"
 #include "common.hpp"
 
@@ -353,6 +355,20 @@ __device__ __forceinline__ void store_tile(const aeisu_product& p, int64_t m0, i
   }
 }
 
+// Lets a kernel have so much LDS on the current device; asked of the runtime once a device.
+template <auto KERNEL>
+hipError_t allow_lds(int bytes) {
+  static std::atomic<uint64_t> allowed;
+  int device = 0;
+  hipError_t e = hipGetDevice(&device);
+  if (e != hipSuccess) return e;
+  const uint64_t bit = uint64_t(1) << (device & 63);
+  if (device < 64 && (allowed.load(std::memory_order_relaxed) & bit)) return hipSuccess;
+  e = hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == hipSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
 // fn<type, result type>: a launch for each pair of them; E4M3 with FP32 results where the kernel has it
 template <bool EXACT, typename Fn>
 hipError_t for_types(const aeisu_product& p, Fn fn) {
@@ -369,12 +385,6 @@ hipError_t for_types(const aeisu_product& p, Fn fn) {
 
 hipError_t launch_product_256(const aeisu_product& p, const int32_t* offsets, int experts, int cus, hipStream_t stream);
 hipError_t launch_product_128(const aeisu_product& p, const int32_t* offsets, int experts, int columns, hipStream_t stream);
-hipError_t launch_product_rows(const aeisu_product& p, const int32_t* offsets, int experts, int mt, int nt, hipStream_t stream);
-
-// Rows of 16-bit operands that do not all start at a multiple of four bytes
-inline bool odd_rows(const aeisu_product& p) {
-  return p.type != AEISU_TYPE_E4M3 && (p.x_stride % 2 || p.w_stride % 2 || p.w_expert_stride % 2 ||
-                                       (reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w)) % 4);
-}
+hipError_t launch_product_rows(const aeisu_product& p, const int32_t* offsets, int experts, int mt, int nt, bool odd, hipStream_t stream);
 
 }  // namespace aeisu
