@@ -10,8 +10,8 @@
 
 Sums are held in FP32 and rounded once to the result's type.  Products of E4M3 operands with an FP32 result are exact;
 with a 16-bit result they may run on the FP8 matrix unit, whose rounding (about 2e-5 of the result) lies below the
-result's own.  All work is enqueued on ``stream`` (default: torch's current one) and nothing waits for it.  Arguments
-that cannot be served raise ``ValueError``.  The HIP kernels of ``libaeisu_amd.so`` do all arithmetic; there is no CPU path.
+result's own.  All work is enqueued on ``stream`` (default: torch's current one) and nothing waits for it; results carry no
+gradient.  Arguments that cannot be served raise ``ValueError``.  The HIP kernels of ``libaeisu_amd.so`` do all arithmetic; there is no CPU path.
 """
 from __future__ import annotations
 
@@ -121,11 +121,12 @@ def _call(device: torch.device, fn, *args) -> None:
 
 
 def _new(shape, dtype, device, stream) -> torch.Tensor:
-    """A result of a call on ``stream``: told to the allocator where that is not the current one."""
-    t = torch.empty(shape, dtype=dtype, device=device)
-    if stream is not None:
-        t.record_stream(stream)
-    return t
+    """A result of a call on ``stream``, from that stream's memory: what the allocator hands out on another stream may
+    still be in use there."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 def quantize_rows(x: torch.Tensor, rows: Optional[torch.Tensor] = None, gated: bool = False,

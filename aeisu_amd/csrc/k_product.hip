@@ -146,8 +146,8 @@ int compute_units() {
 // and 16 a x 16 b with k split over a block's waves (0.34 + 0.60 a + 0.70 b + 0.13 a b) / 32 a step and block of all CUs:
 // 1 x 4096 x 4096 6.4 (a 1, b 1) against 26 for 128 x 128 and 42 for 256 x 256; 100 x 4096 x 4096 8.6 (a 4, b 2) against 26 for
 // 128 x 128; 512 x 4096 x 4096 26 (a 4, b 4) against 20 for 128 x 64.
-// FP32 results of E4M3 operands are exact products on the FP16 unit (128 x 128: 1.79 times the steps, 128 x 64: 1.32);
-// 256 x 256 does not have the registers for their operands.  Few rows at odd elements: 3.6 times the steps (777 x 515 x 1003
+// FP32 results of E4M3 operands are exact products on the FP16 unit (128 x 128: 1.85 times the steps, 128 x 64: 1.4;
+// 8192 x 10240 x 5120: 810 and 899 us); 256 x 256 does not have the registers for their operands.  Few rows at odd elements: 3.6 times the steps (777 x 515 x 1003
 // FP16 over 7 experts: 18.4 with a 2, b 2, 16.5 through registers), and no registers for a 4, b 4.
 // Grouped rows: most experts' last tile is partly filled; 0.97 tiles for each that may have rows matched best.
 // Over 301 shapes of all types, plain and grouped, the kernel chosen so took 2.9 % longer than the best one (geometric
@@ -190,7 +190,7 @@ Choice choose(const aeisu_product& p, bool grouped, int experts, int cus) {
       offer(4.2 + steps * step * slow * std::max(1.0, x) + (0.2 + 0.117 * mt * nt) * x, Choice{Choice::kRows, mt, nt, odd});
     }
   if (near(256)) {
-    const double slow64 = exact ? 1.32 : 1.0, slow128 = exact ? 1.79 : 1.0;
+    const double slow64 = exact ? 1.4 : 1.0, slow128 = exact ? 1.85 : 1.0;
     offer(tiles(share(128, 64), 0.37 * slow64, 0.39 * slow64, 0.53, 3), Choice{Choice::k128, 0, 64, false});
     offer(tiles(share(128, 128), 0.60 * slow128, 0.585 * slow128, 1.0, 2), Choice{Choice::k128, 0, 128, false});
     if (!exact) offer(tiles(share(256, 256), 1.38, 1.38, 5.7, 1), Choice{Choice::k256, 0, 0, false});

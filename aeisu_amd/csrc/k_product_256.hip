@@ -1,9 +1,31 @@
 // Products in tiles of 256 x 256: eight waves of 128 x 64, two groups that multiply and read in turn.
+//
+// A step (128 bytes of k) of a tile is 64 KB of operands and 2048 cycles of the matrix units; two steps fit LDS.  Each SIMD
+// has one wave of either group.  A group's step has four phases, each ended by a barrier of the block: it reads w and half
+// of its rows of x from LDS (L1), multiplies them (M1), reads the other half (L2), multiplies (M2); the second group is
+// one phase behind, so one of them feeds the matrix unit while the other reads.  What each phase frees is filled for the
+// step after next: w after both groups' L1, a group's rows of x after its L2.
+//
+//   phase      0            1            2            3
+//   group 0    L1, x(s+1)   M1           L2, w(s+2)   M2, waits for x(s+1)
+//   group 1    M2 of s-1    L1, x(s+1)   M1           L2, w(s+2), waits for w(s+1)
+//
+// E4M3: the matrix unit sums a step's 128 products from zero and an FMA adds the sum, scaled, three products later, in the
+// shadow of the following ones.  Each sum of 8 products keeps 13 bits below the largest (2e-5 of the result, measured),
+// below the rounding of a 16-bit result; FP32 results take exact products elsewhere.
+// Blocks stay on a CU and take tile after tile; the first two steps of the next are on their way while one is stored.
+//
+// Measured, 8192 x 10240 x 5120 (five tiles on each CU): E4M3 to BF16 339 us, 2,540 TFLOP/s; BF16 567 us, 1,517 TFLOP/s
+// (a library's E4M3 product of 8192 cubed with one scale each reaches 3,022, its BF16 product 1,210).  All waves in one phase:
+// 450 and 722 us.  Loads alone 290 us (L2, 12 TB/s), matrix units 63 % busy, the stores 7 us for each round of tiles at the
+// rate of memory; staggered rounds, wave priorities, waits that pass over the stores and stores past the caches
+// changed nothing.
 #include "product.hpp"
 
 namespace aeisu {
 namespace {
 
+// Loads are counted, not waited for one by one: barrier_behind() lets the youngest be under way.
 template <int TYPE, int OUT>
 __global__ __launch_bounds__(512, 2) void product_phased_kernel(aeisu_product p, const int32_t* offsets, int experts, int ntiles) {
   constexpr bool kE4M3 = TYPE == AEISU_TYPE_E4M3;

