@@ -134,6 +134,19 @@ def test_gate_at_the_ends_of_its_range(B):
     assert v[0] == 0 and v[1] == 0 and v[6] == pytest.approx(2e30, rel=1e-6)
 
 
+def test_gate_of_large_products_whose_logistic_underflows(B):
+    """exp(a) below the normal numbers of FP32, and above them with b: the result is a normal number and keeps 2^-20."""
+    x = torch.cat([-(85 + 80 * torch.rand(40, 128)), 1e38 * (1 + torch.rand(40, 128))], 1)
+    x[:, :128] = x[:, :1] + 0.25 * torch.rand(40, 128)
+    d = x.double()
+    y = (d[:, :128].exp() / (1 + d[:, :128].exp()) * d[:, :128] * d[:, 128:]).numpy()
+    y, x = y[np.abs(y).max(1) > 2.0 ** -100], x[np.abs(y).max(1) > 2.0 ** -100]
+    assert len(y) >= 10
+    q = B.quantize_rows(x.cuda(), gated=True)
+    _, scales = O.quantize(y, 1)
+    assert (np.abs(q.scales.cpu().double().numpy().T - scales) <= scales * 2.0 ** -20).all()
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 @pytest.mark.parametrize("shape", [(1, 1), (128, 128), (129, 257), (3, 70, 130), (2, 300, 128), (4, 1, 500)])
 def test_quantize_weight_is_the_definition(B, shape, dtype):
