@@ -35,7 +35,8 @@ class Product(ctypes.Structure):
     """aeisu_product"""
     _fields_ = [("type", _I), ("out_type", _I), ("rows", _L), ("n", _L), ("k", _L), ("x", _P), ("x_stride", _L),
                 ("x_scales", _P), ("x_scales_stride", _L), ("w", _P), ("w_stride", _L), ("w_expert_stride", _L),
-                ("w_scales", _P), ("bias", _P), ("slope", _F), ("out", _P), ("out_stride", _L)]
+                ("w_scales", _P), ("bias", _P), ("slope", _F), ("out", _P), ("out_stride", _L),
+                ("workspace", _P), ("workspace_bytes", _L)]
 
 
 SIGNATURES = {
@@ -62,6 +63,7 @@ SIGNATURES = {
     "aeisu_destroy": (None, [_P]),
     "aeisu_quantize_rows": (_I, [_P, _I, _L, _L, _L, _I, _P, _L, _P, _L, _P, _L, _P]),
     "aeisu_quantize_weight": (_I, [_P, _I, _L, _L, _L, _L, _L, _P, _P, _P]),
+    "aeisu_product_workspace": (_L, [_P, _L]),
     "aeisu_matmul": (_I, [_P, _P]),
     "aeisu_grouped_matmul": (_I, [_P, _P, _L, _P]),
     "aeisu_last_error": (ctypes.c_char_p, []),

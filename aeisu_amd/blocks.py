@@ -10,8 +10,8 @@
 
 Sums are held in FP32 and rounded once to the result's type.  Products of E4M3 operands with an FP32 result are exact;
 with a 16-bit result they may run on the FP8 matrix unit, whose rounding (about 2e-5 of the result) lies below the
-result's own.  All work is enqueued on ``stream`` (default: torch's current one) and nothing waits for it; results carry no
-gradient.  Arguments that cannot be served raise ``ValueError``.  The HIP kernels of ``libaeisu_amd.so`` do all arithmetic; there is no CPU path.
+result's own.  All work is enqueued on ``stream`` (default: torch's current one) and nothing waits for it; results, and a workspace
+where a product needs one, come from that stream's memory.  Results carry no gradient.  Arguments that cannot be served raise ``ValueError``.  The HIP kernels of ``libaeisu_amd.so`` do all arithmetic; there is no CPU path.
 """
 from __future__ import annotations
 
@@ -177,7 +177,7 @@ def quantize_weight(w: torch.Tensor, stream: Optional[torch.cuda.Stream] = None)
     return QuantWeight(codes, scales, k)
 
 
-_descriptor = struct.Struct("@iiqqqPqPqPqqPPfPq")       # aeisu_product
+_descriptor = struct.Struct("@iiqqqPqPqPqqPPfPqPq")     # aeisu_product
 
 
 def _product(x, w, offsets, bias, slope, out_dtype, out, stream) -> torch.Tensor:
@@ -228,13 +228,19 @@ def _product(x, w, offsets, bias, slope, out_dtype, out, stream) -> torch.Tensor
         raise ValueError(f"offsets are {wshape[0] + 1} contiguous int32 numbers on x's device, of at least one expert")
     if m == 0 or n == 0:
         return out
-    p = _descriptor.pack(kind, _TYPES[out_dtype], m, n, k, xt.data_ptr(), xstride[0], x_scales, x_scales_stride, wt.data_ptr(),
-                         wstride[-2], 0 if offsets is None else wstride[0], w_scales, 0 if bias is None else bias.data_ptr(),
-                         slope, out.data_ptr(), ostride)
+    x_at, w_at, experts = xt.data_ptr(), wt.data_ptr(), 0 if offsets is None else wshape[0]
+    w_strides = wstride[-2], 0 if offsets is None else wstride[0]
+    args = (kind, _TYPES[out_dtype], m, n, k, x_at, xstride[0], x_scales, x_scales_stride, w_at, *w_strides, w_scales,
+            0 if bias is None else bias.data_ptr(), slope, out.data_ptr(), ostride)
+    lib, workspace, need = L.lib(), None, 0
+    if kind != L.TYPE_E4M3 and ((x_at | w_at) & 15 or (k | xstride[0] | w_strides[0] | w_strides[1]) & 7):
+        need = lib.aeisu_product_workspace(_descriptor.pack(*args, 0, 0), experts)   # rows that pay for being laid out first
+        workspace = _new((need,), torch.uint8, device, stream) if need else None
+    p = _descriptor.pack(*args, workspace.data_ptr() if need else 0, need)
     if offsets is None:
-        _call(device, L.lib().aeisu_matmul, p, _stream(device, stream))
+        _call(device, lib.aeisu_matmul, p, _stream(device, stream))
     else:
-        _call(device, L.lib().aeisu_grouped_matmul, p, offsets.data_ptr(), wshape[0], _stream(device, stream))
+        _call(device, lib.aeisu_grouped_matmul, p, offsets.data_ptr(), experts, _stream(device, stream))
     return out
 
 

@@ -47,6 +47,7 @@ void check_product(const aeisu_product& p, int64_t experts) {
   require(p.out && aligned(p.out, os), "product: null or misaligned result");
   require_stride(p.out_stride, p.n, p.rows, "product: the result's row stride is below n");
   require(!p.bias || aligned(p.bias, 4), "product: misaligned bias");
+  require(p.workspace_bytes >= 0 && (!p.workspace || aligned(p.workspace, 16)), "product: misaligned workspace or negative size");
   if (p.k == 0) return;
   require(p.x && p.w && aligned(p.x, es) && aligned(p.w, es), "product: null or misaligned operand");
   require_stride(p.x_stride, kp, p.rows, "product: x's row stride is below its (padded) columns");
@@ -117,6 +118,17 @@ int aeisu_quantize_weight(const void* d_w, int type, int64_t experts, int64_t n,
     const QuantizeWeight q{d_w, n, k, expert_stride, row_stride, static_cast<uint8_t*>(d_codes), d_scales};
     check_launch(launch_quantize_weight(q, type, experts, (hipStream_t)stream), "quantize_weight", (hipStream_t)stream);
   });
+}
+
+int64_t aeisu_product_workspace(const aeisu_product* p, int64_t experts) {
+  int64_t bytes = 0;
+  guarded([&] {
+    require(p != nullptr, "null product");
+    require(experts >= 0 && experts <= 65535, "grouped product: 1 to 65535 experts");
+    check_product(*p, experts);
+    if (p->rows && p->n && p->k) bytes = product_workspace(*p, experts > 0, int(experts > 0 ? experts : 1));
+  });
+  return bytes;
 }
 
 int aeisu_matmul(const aeisu_product* p, void* stream) {

@@ -30,6 +30,8 @@ struct QuantizeWeight {
 };
 hipError_t launch_quantize_weight(const QuantizeWeight& q, int type, int64_t experts, hipStream_t stream);
 
+// Bytes of workspace that the product runs faster with, 0: none
+int64_t product_workspace(const aeisu_product& p, bool grouped, int experts);
 // offsets: null for one weight
 hipError_t launch_product(const aeisu_product& p, const int32_t* offsets, int experts, hipStream_t stream);
 

@@ -156,7 +156,14 @@ struct Choice {
   enum { kAny, k128, k256, kRows } kernel;
   int mt, nt;                                        // kRows: a, b; k128: columns
   bool odd;                                          // kRows: from memory into registers
+  double us = 0;                                     // expected
 };
+// 16-byte pieces of rows: what LDS takes from memory
+bool whole_pieces(const aeisu_product& p) {
+  return p.type == AEISU_TYPE_E4M3 ||
+         (p.k % 8 == 0 && p.x_stride % 8 == 0 && p.w_stride % 8 == 0 && p.w_expert_stride % 8 == 0 &&
+          (reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w)) % 16 == 0);
+}
 Choice choose(const aeisu_product& p, bool grouped, int experts, int cus) {
   const bool e4m3 = p.type == AEISU_TYPE_E4M3, exact = e4m3 && p.out_type == AEISU_TYPE_F32;
   const int64_t es = e4m3 ? 1 : 2;
@@ -176,9 +183,7 @@ Choice choose(const aeisu_product& p, bool grouped, int experts, int cus) {
   auto offer = [&](double t, Choice c) {
     if (t < least) least = t, best = c;
   };
-  // 16-byte pieces of rows, and 32-bit offsets within a tile
-  const bool pieces = e4m3 || (p.k % 8 == 0 && p.x_stride % 8 == 0 && p.w_stride % 8 == 0 && p.w_expert_stride % 8 == 0 &&
-                               (reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w)) % 16 == 0);
+  const bool pieces = whole_pieces(p);               // and 32-bit offsets within a tile
   const int64_t apart = std::max(p.x_stride, p.w_stride) * es;
   auto near = [&](int rows) { return pieces && apart <= (int64_t(1) << 32) / rows - kStepBytes; };
   const double slow = exact ? 1.14 : e4m3 ? 1.0 : pieces ? 1.07 : 3.6;
@@ -195,20 +200,108 @@ Choice choose(const aeisu_product& p, bool grouped, int experts, int cus) {
     offer(tiles(share(128, 128), 0.60 * slow128, 0.585 * slow128, 1.0, 2), Choice{Choice::k128, 0, 128, false});
     if (!exact) offer(tiles(share(256, 256), 1.38, 1.38, 5.7, 1), Choice{Choice::k256, 0, 0, false});
   }
+  best.us = least;
   return best;
 }
 
-}  // namespace
+// Operands laid out for whole pieces: rows of 16-bit values to 16-byte aligned ones, filled up with zeros to a multiple of 8
+// columns.  One pass over x and then w, sixteen lanes a row and 128 columns, two of these a thread.
+struct LayOut {
+  struct Operand {
+    const char* from;
+    char* to;
+    unsigned rows, group;                            // in all, and of an expert
+    int64_t group_stride, stride;                    // bytes
+  } x, w;
+  int cols, padded;
+};
+__global__ __launch_bounds__(256) void lay_out_kernel(LayOut l, unsigned x_blocks) {
+  const bool is_x = blockIdx.x < x_blocks;
+  const LayOut::Operand o = is_x ? l.x : l.w;
+  const unsigned r = (blockIdx.x - (is_x ? 0 : x_blocks)) * 16 + (threadIdx.x >> 4);
+  if (r >= o.rows) return;
+  const unsigned g = r / o.group;
+  const char* from = o.from + (int64_t)g * o.group_stride + (int64_t)(r - g * o.group) * o.stride;
+  char* to = o.to + (int64_t)r * l.padded * 2;
+  const int c0 = (int)blockIdx.y * 256 + (int)(threadIdx.x & 15) * 8;
+  Piece<2, true> v[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int c = c0 + i * 128;
+    v[i] = load_piece<2, true>(from + (int64_t)c * 2, l.cols - c, c > 0);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (c0 + i * 128 < l.padded) *reinterpret_cast<i4*>(to + (int64_t)(c0 + i * 128) * 2) = v[i].whole();
+}
 
-hipError_t launch_product(const aeisu_product& p, const int32_t* offsets, int experts, hipStream_t stream) {
-  const int cus = compute_units();
-  const Choice c = choose(p, offsets != nullptr, experts, cus);
+// The product on operands laid out in a workspace, and the bytes of it.
+struct Laid {
+  aeisu_product p;
+  LayOut l;
+  int64_t x_bytes, bytes;
+};
+bool lay_out(const aeisu_product& p, int experts, Laid& r) {
+  if (p.type == AEISU_TYPE_E4M3 || whole_pieces(p)) return false;
+  const int64_t padded = (p.k + 7) / 8 * 8, weights = p.w_expert_stride == 0 ? 1 : experts;
+  if (p.rows + weights * p.n > int64_t(1) << 27 || padded > 65535 * 256) return false;   // the grid's limits
+  r.x_bytes = (p.rows * padded * 2 + 255) / 256 * 256;
+  r.bytes = r.x_bytes + weights * p.n * padded * 2;
+  char* to = static_cast<char*>(p.workspace);
+  r.l.x = {static_cast<const char*>(p.x), to, (unsigned)p.rows, (unsigned)p.rows, 0, p.x_stride * 2};
+  r.l.w = {static_cast<const char*>(p.w), to ? to + r.x_bytes : nullptr, (unsigned)(weights * p.n), (unsigned)p.n,
+           p.w_expert_stride * 2, p.w_stride * 2};
+  r.l.cols = (int)p.k;
+  r.l.padded = (int)padded;
+  r.p = p;
+  r.p.x = r.l.x.to;
+  r.p.w = r.l.w.to;
+  r.p.x_stride = r.p.w_stride = r.p.k = padded;
+  r.p.w_expert_stride = weights == 1 ? 0 : p.n * padded;
+  return true;
+}
+// Whether that pays, and the kernel of either way.  Laying out takes 6 us (a launch and the wait for it) and each byte read
+// and written at 4.5 TB/s.  BF16 of odd k, whole calls without and with it: 16,384 x 4000 x 4001 over 4 experts 1561 and 560 us
+// (449 on aligned rows), 16,384 x 2047 x 2049 over 8 446 and 171, 6000 x 2816 x 2047 over 16 269 and 182, 2000 x 2000 x 1501
+// over 2 49 and 33; where weights outweigh the rows it loses: 100 x 3000 x 3333 over 30 156 and about 270, and where the product
+// is small: 777 x 515 x 1003 over 7 16.5 and 19.9.
+bool laid_pays(const Laid& r, bool grouped, int experts, int cus, const Choice& direct, Choice& then) {
+  then = choose(r.p, grouped, experts, cus);
+  return then.us + 6.0 + 2.0 * double(r.bytes) / 4.5e6 < direct.us;
+}
+
+hipError_t launch(const aeisu_product& p, const int32_t* offsets, int experts, int cus, const Choice& c, hipStream_t stream) {
   switch (c.kernel) {
     case Choice::k256: return launch_product_256(p, offsets, experts, cus, stream);
     case Choice::k128: return launch_product_128(p, offsets, experts, c.nt, stream);
     case Choice::kRows: return launch_product_rows(p, offsets, experts, c.mt, c.nt, c.odd, stream);
     default: return launch_product_any(p, offsets, experts, stream);
   }
+}
+
+}  // namespace
+
+int64_t product_workspace(const aeisu_product& p, bool grouped, int experts) {
+  aeisu_product q = p;
+  q.workspace = nullptr;
+  Laid r;
+  Choice then;
+  const int cus = compute_units();
+  return lay_out(q, experts, r) && laid_pays(r, grouped, experts, cus, choose(p, grouped, experts, cus), then) ? r.bytes : 0;
+}
+
+hipError_t launch_product(const aeisu_product& p, const int32_t* offsets, int experts, hipStream_t stream) {
+  const int cus = compute_units();
+  Choice c = choose(p, offsets != nullptr, experts, cus), then;
+  Laid r;
+  if (p.workspace && lay_out(p, experts, r) && r.bytes <= p.workspace_bytes &&
+      laid_pays(r, offsets != nullptr, experts, cus, c, then)) {
+    const unsigned x_blocks = (r.l.x.rows + 15) / 16, w_blocks = (r.l.w.rows + 15) / 16;
+    lay_out_kernel<<<dim3(x_blocks + w_blocks, (r.l.padded + 255) / 256), 256, 0, stream>>>(r.l, x_blocks);
+    const hipError_t e = hipGetLastError();
+    return e != hipSuccess ? e : launch(r.p, offsets, experts, cus, then, stream);
+  }
+  return launch(p, offsets, experts, cus, c, stream);
 }
 
 }  // namespace aeisu

@@ -243,7 +243,14 @@ typedef struct aeisu_product {
   float slope;                           /* finite, >= 0 */
   void* out;                             /* [rows][out_stride] */
   int64_t out_stride;
+  void* workspace;                       /* 16-byte aligned, or NULL; used where aeisu_product_workspace asks for it */
+  int64_t workspace_bytes;
 } aeisu_product;
+
+/* Bytes of workspace with which this product (its workspace apart; experts 0: aeisu_matmul) runs faster than without: large
+ * ones of F16 / BF16 operands whose rows are not 16-byte aligned or no multiple of 8 columns are laid out there first.
+ * 0: none, also for a product that would be refused. */
+int64_t aeisu_product_workspace(const aeisu_product* p, int64_t experts);
 
 int aeisu_matmul(const aeisu_product* p, void* stream);
 

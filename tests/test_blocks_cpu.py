@@ -46,6 +46,29 @@ def test_grouped_products_are_refused():
     assert lib.aeisu_matmul(None, None) == L.AEISU_ERR_INVALID_ARGUMENT
 
 
+def test_workspaces_are_checked_and_asked_for():
+    """A workspace has to be aligned; it is asked for by large 16-bit products out of line, and by no other."""
+    lib = L.lib()
+    for change in ({"workspace": P + 8, "workspace_bytes": 64}, {"workspace": P, "workspace_bytes": -1}):
+        p = product(**change)
+        assert lib.aeisu_matmul(ctypes.byref(p), None) == L.AEISU_ERR_INVALID_ARGUMENT
+        assert "workspace" in lib.aeisu_last_error().decode()
+
+    def need(experts=4, **change):
+        v = dict(type=L.TYPE_BF16, rows=16000, n=2000, k=2000, x_stride=2000, w_stride=2000, w_expert_stride=4000000, out_stride=2000)
+        v.update(change)
+        return lib.aeisu_product_workspace(ctypes.byref(product(**v)), experts)
+    assert need() == 0                                                     # in line
+    assert need(k=1999) == (16000 + 4 * 2000) * 2000 * 2                   # columns that end inside a piece
+    assert need(x=P + 2) == need(w=P + 2) == need(k=1999)                  # rows that start inside one
+    assert need(k=1999, w_expert_stride=0) == (16000 + 2000) * 2000 * 2    # one weight for all
+    assert need(k=1999, rows=2) == 0                                       # less work than laying out
+    assert need(k=1999, x_stride=100) == 0 and need(k=1999, experts=70000) == 0 and need(k=1999, rows=0) == 0
+    assert need(0, k=1999) == (16000 + 2000) * 2000 * 2                    # one weight, no offsets
+    assert lib.aeisu_product_workspace(None, 4) == 0
+    assert lib.aeisu_product_workspace(ctypes.byref(product(rows=16000)), 4) == 0
+
+
 def test_nothing_to_do_is_no_error():
     lib = L.lib()
     assert lib.aeisu_matmul(ctypes.byref(product(rows=0, x=0, w=0, out=0)), None) == L.AEISU_OK

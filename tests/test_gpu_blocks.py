@@ -416,6 +416,62 @@ def test_large_grouped_matmul(B, counts, kind, k, out_dtype):
     O.check(out[:t], y.cpu(), mag.cpu(), k, kind == "e4m3", f"{counts[:3]} {kind} {k}")
 
 
+@pytest.mark.parametrize("kind,out_dtype", [("f16", F16), ("bf16", F32), ("f16", F32)])
+@pytest.mark.parametrize("counts,n,k", [([700, 0, 1500, 1, 300], 900, 1001), ([3000, 1100], 515, 2003), ([257] * 9, 1300, 1150),
+                                        ([5000], 1030, 777), ([7000, 0, 4000, 1, 1000], 900, 1001), ([3000, 3000, 1000], 1500, 1100)])
+def test_large_products_on_rows_that_are_laid_out(B, counts, n, k, kind, out_dtype):
+    """Rows and weights at odd addresses with NaN round them, on both sides of where laying them out pays (there for
+    certain from five million results on): with the workspace that the library asks for, one that is too small, and none."""
+    from aeisu_amd import _lib as L
+    import ctypes
+    e, t, dtype = len(counts), sum(counts), F16 if kind == "f16" else BF16
+    g = torch.Generator("cuda").manual_seed(k)
+    xb = torch.full((t + 2, k + 4), float("nan"), dtype=dtype, device="cuda")
+    wb = torch.full((e, n + 2, k + 5), float("nan"), dtype=dtype, device="cuda")
+    x, w = xb[1:t + 1, 3:k + 3], wb[:, 1:n + 1, 1:k + 1]
+    x.copy_(torch.randn(t, k, generator=g, device="cuda"))
+    w.copy_(torch.randn(e, n, k, generator=g, device="cuda"))
+    bias, off = torch.randn(e, n, generator=g, device="cuda"), offsets_of(counts)
+    y = torch.cat([v.double() @ wi.double().t() + b.double() for v, wi, b in zip(x.split(counts), w, bias)])
+    mag = torch.cat([v.double().abs() @ wi.double().abs().t() + b.double().abs() for v, wi, b in zip(x.split(counts), w, bias)])
+    y = torch.where(y < 0, y * 0.25, y)
+    got = B.grouped_matmul(x, w, off, bias=bias, slope=0.25, out_dtype=out_dtype)
+    O.check(got, y.cpu(), mag.cpu(), k, False, "with the workspace asked for")
+    assert torch.equal(got, B.grouped_matmul(x, w, off, bias=bias, slope=0.25, out_dtype=out_dtype))
+    room = torch.empty((t, n), dtype=out_dtype, device="cuda")
+    p = L.Product(type=B._TYPES[dtype], out_type=B._TYPES[out_dtype], rows=t, n=n, k=k, x=x.data_ptr(), x_stride=x.stride(0),
+                  w=w.data_ptr(), w_stride=w.stride(1), w_expert_stride=w.stride(0), bias=bias.data_ptr(), slope=0.25,
+                  out=room.data_ptr(), out_stride=n)
+    need = L.lib().aeisu_product_workspace(ctypes.byref(p), e)
+    padded = -(-k // 8) * 8
+    assert need in (0, -(-t * padded * 2 // 256) * 256 + e * n * padded * 2) and (need or t * n < 5000000)
+    for size in (need, need - 1, 0) if need else (0,):
+        space = torch.full((need + 256,), 255, dtype=torch.uint8, device="cuda")
+        p.workspace, p.workspace_bytes = space.data_ptr() if size else 0, size
+        room.fill_(float("nan"))
+        L.check(L.lib().aeisu_grouped_matmul(ctypes.byref(p), off.data_ptr(), e, torch.cuda.current_stream().cuda_stream))
+        O.check(room, y.cpu(), mag.cpu(), k, False, f"workspace of {size}")
+        assert (space[need if size == need else 0:] == 255).all()
+        assert size < need or torch.equal(room, got)
+
+
+def test_laid_out_rows_of_one_weight_for_all_experts(B):
+    """A weight of expert stride 0, and operands of which only one is out of line."""
+    t, e, n, k = 4000, 6, 1000, 1024
+    g = torch.Generator("cuda").manual_seed(9)
+    x, one = (torch.randn(r, k, generator=g, device="cuda").bfloat16() for r in (t, n))
+    w, off = one.expand(e, n, k), offsets_of([900, 0, 1100, 1000, 999, 1])
+    want = x.double() @ one.double().t()
+    mag = x.double().abs() @ one.double().abs().t()
+    shifted = torch.full((t, k + 1), float("nan"), dtype=BF16, device="cuda")[:, 1:]
+    shifted.copy_(x)
+    for a in (x, shifted):
+        O.check(B.grouped_matmul(a, w, off, out_dtype=F32), want.cpu(), mag.cpu(), k, False, "one weight")
+    short = x[:, :1021], w[:, :, :1021]              # aligned rows whose columns end inside a piece
+    want, mag = short[0].double() @ one[:, :1021].double().t(), short[0].double().abs() @ one[:, :1021].double().abs().t()
+    O.check(B.grouped_matmul(*short, off, out_dtype=F32), want.cpu(), mag.cpu(), 1021, False, "short rows")
+
+
 # ---- memory, streams, graphs ------------------------------------------------------------------------------------
 def test_offsets_past_32_bits(B):
     """Operands and results whose rows lie more than 4 GiB apart from first to last."""
