@@ -124,9 +124,9 @@ def _new(shape, dtype, device, stream) -> torch.Tensor:
     """A result of a call on ``stream``, from that stream's memory: what the allocator hands out on another stream may
     still be in use there."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return torch.empty(*shape, dtype=dtype, device=device)     # sizes one by one: a tuple takes 0.5 us more to parse
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return torch.empty(*shape, dtype=dtype, device=device)
 
 
 def quantize_rows(x: torch.Tensor, rows: Optional[torch.Tensor] = None, gated: bool = False,
@@ -157,7 +157,9 @@ def quantize_rows(x: torch.Tensor, rows: Optional[torch.Tensor] = None, gated: b
     if n and k:
         _call(device, L.lib().aeisu_quantize_rows, x.data_ptr(), dtype, m, x.stride(0), k, gated, index, n, codes.data_ptr(),
               kb * BLOCK, scales.data_ptr(), n, _stream(device, stream))
-    return QuantRows(codes, scales, k)
+    q = QuantRows.__new__(QuantRows)                     # nothing to check
+    q.codes, q.scales, q.cols = codes, scales, k
+    return q
 
 
 def quantize_weight(w: torch.Tensor, stream: Optional[torch.cuda.Stream] = None) -> QuantWeight:
@@ -178,6 +180,7 @@ def quantize_weight(w: torch.Tensor, stream: Optional[torch.cuda.Stream] = None)
 
 
 _descriptor = struct.Struct("@iiqqqPqPqPqqPPfPqPq")     # aeisu_product
+_workspace = struct.Struct("@Pq")                       # its last two members
 
 
 def _product(x, w, offsets, bias, slope, out_dtype, out, stream) -> torch.Tensor:
@@ -228,15 +231,16 @@ def _product(x, w, offsets, bias, slope, out_dtype, out, stream) -> torch.Tensor
         raise ValueError(f"offsets are {wshape[0] + 1} contiguous int32 numbers on x's device, of at least one expert")
     if m == 0 or n == 0:
         return out
-    x_at, w_at, experts = xt.data_ptr(), wt.data_ptr(), 0 if offsets is None else wshape[0]
-    w_strides = wstride[-2], 0 if offsets is None else wstride[0]
-    args = (kind, _TYPES[out_dtype], m, n, k, x_at, xstride[0], x_scales, x_scales_stride, w_at, *w_strides, w_scales,
-            0 if bias is None else bias.data_ptr(), slope, out.data_ptr(), ostride)
-    lib, workspace, need = L.lib(), None, 0
-    if kind != L.TYPE_E4M3 and ((x_at | w_at) & 15 or (k | xstride[0] | w_strides[0] | w_strides[1]) & 7):
-        need = lib.aeisu_product_workspace(_descriptor.pack(*args, 0, 0), experts)   # rows that pay for being laid out first
-        workspace = _new((need,), torch.uint8, device, stream) if need else None
-    p = _descriptor.pack(*args, workspace.data_ptr() if need else 0, need)
+    x_at, w_at, wrow = xt.data_ptr(), wt.data_ptr(), wstride[-2]
+    experts, wexpert = (0, 0) if offsets is None else (wshape[0], wstride[0])
+    p = _descriptor.pack(kind, _TYPES[out_dtype], m, n, k, x_at, xstride[0], x_scales, x_scales_stride, w_at, wrow, wexpert, w_scales,
+                         0 if bias is None else bias.data_ptr(), slope, out.data_ptr(), ostride, 0, 0)
+    lib = L.lib()
+    if kind != L.TYPE_E4M3 and ((x_at | w_at) & 15 or (k | xstride[0] | wrow | wexpert) & 7):
+        need = lib.aeisu_product_workspace(p, experts)             # bytes, where the rows pay for being laid out first
+        if need:
+            workspace = _new((need,), torch.uint8, device, stream)
+            p = p[:-_workspace.size] + _workspace.pack(workspace.data_ptr(), need)
     if offsets is None:
         _call(device, lib.aeisu_matmul, p, _stream(device, stream))
     else:
