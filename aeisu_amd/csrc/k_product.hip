@@ -13,19 +13,21 @@
 namespace aeisu {
 namespace {
 
-// 64 x 64 tiles of the result, one for each block of four waves (2 x 2, each 32 x 32); operands staged through registers,
-// so rows may start at any address and end anywhere.  The pieces of the AHEAD steps after the one that is multiplied
-// are on their way into registers, and LDS holds two steps.
-template <int TYPE>
-__global__ __launch_bounds__(256) void product_kernel(aeisu_product p, const int32_t* offsets, int experts, int64_t ntiles) {
+// 64 x 64 tiles of the result, one for each block; operands staged through registers, so rows may start at any address and
+// end anywhere.  Four waves (2 x 2, each 32 x 32) take a step; with SPLIT 2 eight waves take two steps at a time and their
+// sums meet in LDS.  The pieces of the AHEAD steps after the one that is multiplied are on their way into registers, and
+// LDS holds two steps of either half.
+template <int TYPE, int SPLIT>
+__global__ __launch_bounds__(256 * SPLIT) void product_kernel(aeisu_product p, const int32_t* offsets, int experts, int64_t ntiles) {
   constexpr int BM = 64, BN = 64, AHEAD = 3;
   constexpr bool kE4M3 = TYPE == AEISU_TYPE_E4M3, ODD = !kE4M3;
   constexpr int ES = kE4M3 ? 1 : 2, PER = 16 / ES, STEP = kStepBytes / ES;
-  __shared__ i4 lds[2][2][BM * 8];                   // step, x or w: row r's eight pieces, exchanged by r & 7
+  __shared__ i4 lds[SPLIT][2][2][BM * 8];            // half, step, x or w: row r's eight pieces, exchanged by r & 7
+  const int part = SPLIT == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), thread = threadIdx.x & 255;
   RowTile tile;
   if (!find_tile<BM>(offsets, experts, p.rows, (int)(blockIdx.x / ntiles), tile)) return;
   const int64_t n0 = (int64_t)(blockIdx.x % ntiles) * BN;
-  const int lane = lane_id(), wave = threadIdx.x >> 6, wm = (wave & 1) * 2, wn = (wave >> 1) * 2;
+  const int lane = lane_id(), wave = thread >> 6, wm = (wave & 1) * 2, wn = (wave >> 1) * 2;
   const int e = tile.expert < 0 ? 0 : tile.expert;
   const int64_t kb = (p.k + kBlock - 1) / kBlock;
   const float* sw = kE4M3 ? p.w_scales + (e * ((p.n + kBlock - 1) / kBlock) + n0 / kBlock) * kb : nullptr;
@@ -40,7 +42,7 @@ __global__ __launch_bounds__(256) void product_kernel(aeisu_product p, const int
   int first[2];                                      // and their first column in a step
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int c = threadIdx.x + 256 * (i & 1), row = c >> 3, piece = c & 7;   // 512 pieces of 16 bytes an operand
+    const int c = thread + 256 * (i & 1), row = c >> 3, piece = c & 7;   // 512 pieces of 16 bytes an operand
     if (i < 2) {
       const int64_t r = tile.lo + row < tile.hi ? tile.lo + row : tile.hi - 1;
       src[i] = static_cast<const char*>(p.x) + r * p.x_stride * ES + piece * 16;
@@ -58,17 +60,20 @@ __global__ __launch_bounds__(256) void product_kernel(aeisu_product p, const int
   };
   Piece<ES, ODD> st[AHEAD][4];
 #pragma unroll
-  for (int u = 0; u < AHEAD; ++u) fetch(u, st[u]);
-  for (int s0 = 0; s0 < steps; s0 += AHEAD) {
+  for (int u = 0; u < AHEAD; ++u) fetch(u * SPLIT + part, st[u]);
+  for (int s0 = 0; s0 < steps; s0 += AHEAD * SPLIT) {
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int s = s0 + u;
-      if (s >= steps) break;
-      i4(&to)[2][BM * 8] = lds[s & 1];               // read last two steps ago, before the barrier of the step before
+      if (s0 + u * SPLIT >= steps) break;
+      const int s = s0 + u * SPLIT + part;           // past the last one: this half only keeps to the barriers
+      i4(&to)[2][BM * 8] = lds[part][(s / SPLIT) & 1];   // read last two steps ago, before the barrier of the step before
+      if (s < steps) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) to[i >> 1][((threadIdx.x >> 3) + 32 * (i & 1)) * 8 + ((threadIdx.x ^ (threadIdx.x >> 3)) & 7)] = st[u][i].whole();
-      fetch(s + AHEAD, st[u]);
+        for (int i = 0; i < 4; ++i) to[i >> 1][((thread >> 3) + 32 * (i & 1)) * 8 + ((thread ^ (thread >> 3)) & 7)] = st[u][i].whole();
+      }
+      fetch(s + AHEAD * SPLIT, st[u]);
       lds_barrier();
+      if (SPLIT > 1 && s >= steps) break;
       Frag x[2], w[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -93,6 +98,17 @@ __global__ __launch_bounds__(256) void product_kernel(aeisu_product p, const int
       }
     }
   }
+  if constexpr (SPLIT == 2) {                        // the second half's sums, 16 KB, over what its own steps held
+    f4* sums = reinterpret_cast<f4*>(&lds[1][0][0][0]);
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (part == 1) sums[i * 256 + thread] = acc[i >> 1][i & 1];
+    lds_barrier();
+    if (part == 1) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] += sums[i * 256 + thread];
+  }
   const size_t vec = p.out_type == AEISU_TYPE_F32 ? 16 : 8;
   const bool wide = (reinterpret_cast<uintptr_t>(p.out) % vec) == 0 && p.out_stride % 4 == 0;
   const float* bias = p.bias && tile.expert >= 0 ? p.bias + (int64_t)e * p.n : nullptr;
@@ -107,14 +123,14 @@ __global__ __launch_bounds__(256) void product_kernel(aeisu_product p, const int
 
 }  // namespace
 
-hipError_t launch_product_any(const aeisu_product& p, const int32_t* offsets, int experts, hipStream_t stream) {
+hipError_t launch_product_any(const aeisu_product& p, const int32_t* offsets, int experts, bool split, hipStream_t stream) {
   const int64_t ntiles = (p.n + 63) / 64;
   const int64_t blocks = most_tiles(p.rows, experts, offsets != nullptr, 64) * ntiles;
   if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
-  auto go = [&](auto kernel) { kernel<<<(unsigned)blocks, 256, 0, stream>>>(p, offsets, experts, ntiles); };
-  if (p.type == AEISU_TYPE_E4M3) go(product_kernel<AEISU_TYPE_E4M3>);
-  else if (p.type == AEISU_TYPE_F16) go(product_kernel<AEISU_TYPE_F16>);
-  else go(product_kernel<AEISU_TYPE_BF16>);
+  auto go = [&](auto kernel, int threads) { kernel<<<(unsigned)blocks, threads, 0, stream>>>(p, offsets, experts, ntiles); };
+  if (p.type == AEISU_TYPE_E4M3) go(product_kernel<AEISU_TYPE_E4M3, 1>, 256);
+  else if (p.type == AEISU_TYPE_F16) split ? go(product_kernel<AEISU_TYPE_F16, 2>, 512) : go(product_kernel<AEISU_TYPE_F16, 1>, 256);
+  else split ? go(product_kernel<AEISU_TYPE_BF16, 2>, 512) : go(product_kernel<AEISU_TYPE_BF16, 1>, 256);
   return hipGetLastError();
 }
 
@@ -154,7 +170,7 @@ int compute_units() {
 // mean).
 struct Choice {
   enum { kAny, k128, k256, kRows } kernel;
-  int mt, nt;                                        // kRows: a, b; k128: columns
+  int mt, nt;                                        // kRows: a, b; k128: columns; kAny: nt steps at a time
   bool odd;                                          // kRows: from memory into registers
   double us = 0;                                     // expected
 };
@@ -178,8 +194,12 @@ Choice choose(const aeisu_product& p, bool grouped, int experts, int cus) {
     const double rounds = std::floor(blocks / on_cu), rest = blocks - rounds * on_cu;
     return 4.5 + rounds * round(on_cu) + (rest > 0 ? round(rest) : 0);
   };
-  Choice best{Choice::kAny, 0, 0, false};
-  double least = tiles(share(64, 64), 0.73, 0.43, 1.2, 4);
+  // Two steps at a time while every block has a CU to itself (16-bit operands: 777 x 515 x 1003 over 7 experts 15.2 us for
+  // 16.4, 400 x 500 x 3001 over 3 26 for 31); only one such block fits a CU, and with two for each CU it is slower
+  // (1500 x 1001 x 1501 over 8 35.7 and 29.2).
+  const bool split = !e4m3 && share(64, 64) <= 1;
+  Choice best{Choice::kAny, 0, split ? 2 : 1, false};
+  double least = tiles(share(64, 64), split ? 0.62 : 0.73, 0.43, 1.2, 4);
   auto offer = [&](double t, Choice c) {
     if (t < least) least = t, best = c;
   };
@@ -264,7 +284,7 @@ bool lay_out(const aeisu_product& p, int experts, Laid& r) {
 // and written at 4.5 TB/s.  BF16 of odd k, whole calls without and with it: 16,384 x 4000 x 4001 over 4 experts 1561 and 560 us
 // (449 on aligned rows), 16,384 x 2047 x 2049 over 8 446 and 171, 6000 x 2816 x 2047 over 16 269 and 182, 2000 x 2000 x 1501
 // over 2 49 and 33; where weights outweigh the rows it loses: 100 x 3000 x 3333 over 30 156 and about 270, and where the product
-// is small: 777 x 515 x 1003 over 7 16.5 and 19.9.
+// is small: 777 x 515 x 1003 over 7 15.2 and 19.9.
 bool laid_pays(const Laid& r, bool grouped, int experts, int cus, const Choice& direct, Choice& then) {
   then = choose(r.p, grouped, experts, cus);
   return then.us + 6.0 + 2.0 * double(r.bytes) / 4.5e6 < direct.us;
@@ -275,7 +295,7 @@ hipError_t launch(const aeisu_product& p, const int32_t* offsets, int experts, i
     case Choice::k256: return launch_product_256(p, offsets, experts, cus, stream);
     case Choice::k128: return launch_product_128(p, offsets, experts, c.nt, stream);
     case Choice::kRows: return launch_product_rows(p, offsets, experts, c.mt, c.nt, c.odd, stream);
-    default: return launch_product_any(p, offsets, experts, stream);
+    default: return launch_product_any(p, offsets, experts, c.nt == 2, stream);
   }
 }
 

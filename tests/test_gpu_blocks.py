@@ -455,6 +455,19 @@ def test_large_products_on_rows_that_are_laid_out(B, counts, n, k, kind, out_dty
         assert size < need or torch.equal(room, got)
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("k", [1003, 1067, 70, 2051])
+def test_products_of_few_rows_out_of_line_in_two_halves(B, kind, k):
+    """One block for each CU at most: two steps at a time, their number odd and even, the last one partly filled."""
+    counts, n = [120, 0, 200, 1, 150, 190, 116], 515
+    off = offsets_of(counts)
+    x, w, bias, xv, wv = grouped_case(B, kind, sum(counts), len(counts), n, k)
+    y, mag = O.grouped(xv, wv, off.tolist(), bias, 0.25)
+    got = B.grouped_matmul(x, w, off, bias=bias, slope=0.25, out_dtype=F32)
+    O.check(got, y, mag, k, False, f"{kind} k {k}")
+    assert torch.equal(got, B.grouped_matmul(x, w, off, bias=bias, slope=0.25, out_dtype=F32))
+
+
 def test_laid_out_rows_of_one_weight_for_all_experts(B):
     """A weight of expert stride 0, and operands of which only one is out of line."""
     t, e, n, k = 4000, 6, 1000, 1024
