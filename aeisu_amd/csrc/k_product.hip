@@ -211,6 +211,7 @@ Choice choose(const aeisu_product& p, bool grouped, int experts, int cus) {
     for (int nt = 1; nt <= (mt == 1 ? 2 : mt); nt *= 2) {
       const bool odd = !near(16 * std::max(mt, nt));
       if (odd && (e4m3 || mt * nt == 16)) continue;
+      if (share(16 * mt, 16 * nt) * cus >= 1 << 22) continue;   // 2^31 threads
       const double x = share(16 * mt, 16 * nt), step = (0.34 + 0.60 * mt + 0.70 * nt + 0.13 * mt * nt) / 32;
       offer(4.2 + steps * step * slow * std::max(1.0, x) + (0.2 + 0.117 * mt * nt) * x, Choice{Choice::kRows, mt, nt, odd});
     }

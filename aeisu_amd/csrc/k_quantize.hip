@@ -253,10 +253,23 @@ hipError_t launch_rows(const QuantizeRows& q, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_quantize_rows(const QuantizeRows& q, int type, bool gated, hipStream_t stream) {
-  if (type == AEISU_TYPE_F16) return gated ? launch_rows<AEISU_TYPE_F16, true>(q, stream) : launch_rows<AEISU_TYPE_F16, false>(q, stream);
-  if (type == AEISU_TYPE_BF16) return gated ? launch_rows<AEISU_TYPE_BF16, true>(q, stream) : launch_rows<AEISU_TYPE_BF16, false>(q, stream);
-  return gated ? launch_rows<AEISU_TYPE_F32, true>(q, stream) : launch_rows<AEISU_TYPE_F32, false>(q, stream);
+hipError_t launch_quantize_rows(const QuantizeRows& all, int type, bool gated, hipStream_t stream) {
+  constexpr int64_t kRows = int64_t(1) << 27;        // rows a launch: 2^31 threads in x
+  const int64_t size = type == AEISU_TYPE_F32 ? 4 : 2;
+  for (int64_t r = 0; r < all.rows; r += kRows) {
+    QuantizeRows q = all;
+    q.rows = all.rows - r < kRows ? all.rows - r : kRows;
+    q.codes += r * all.codes_stride;
+    q.scales += r;
+    if (all.index) q.index += r;
+    else q.x = static_cast<const char*>(all.x) + r * all.x_stride * size, q.x_rows -= r;
+    hipError_t e;
+    if (type == AEISU_TYPE_F16) e = gated ? launch_rows<AEISU_TYPE_F16, true>(q, stream) : launch_rows<AEISU_TYPE_F16, false>(q, stream);
+    else if (type == AEISU_TYPE_BF16) e = gated ? launch_rows<AEISU_TYPE_BF16, true>(q, stream) : launch_rows<AEISU_TYPE_BF16, false>(q, stream);
+    else e = gated ? launch_rows<AEISU_TYPE_F32, true>(q, stream) : launch_rows<AEISU_TYPE_F32, false>(q, stream);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_quantize_weight(const QuantizeWeight& q, int type, int64_t experts, hipStream_t stream) {

@@ -510,6 +510,24 @@ def test_offsets_past_32_bits(B):
     assert torch.equal(B.grouped_matmul(src, w16, off), B.grouped_matmul(src.contiguous(), w16, off))
 
 
+@pytest.mark.parametrize("gathered", [False, True])
+def test_more_rows_than_a_launch_takes(B, gathered):
+    """2^27 rows and some: both sides of where the second launch begins."""
+    first, more = 1 << 27, 37
+    x = torch.empty(1000 if gathered else first + more, 3, dtype=F16, device="cuda")
+    x[:1000].normal_()
+    x[-1000:].normal_()
+    index = None
+    if gathered:
+        index = torch.full((first + more,), -1, dtype=torch.int32, device="cuda")
+        index[:500] = torch.arange(500, device="cuda", dtype=torch.int32)
+        index[-500:] = torch.arange(999, 499, -1, device="cuda", dtype=torch.int32)
+    q = B.quantize_rows(x, rows=index)
+    for part in (slice(0, 500), slice(first + more - 500, first + more)):
+        want = B.quantize_rows(x[index[part].long()] if gathered else x[part])
+        assert torch.equal(q.codes[part], want.codes) and torch.equal(q.scales[:, part], want.scales)
+
+
 def test_work_is_ordered_on_the_given_stream(B):
     x, w, _ = operands(B, 300, 400, 1000)
     src = tensor(values(rng(3), 300, 1000), BF16)
